@@ -600,6 +600,115 @@ int kn_multimatmul_A_transposed(const float* A, int64_t a_cols, const float* B, 
 /* cuda/render_to_screen.cpp:222-248 — OpenGL viewer: not supported. */
 int kn_render_to_screen(void);
 
+/* ---------------------------------------------------------------------------
+ * Gated experts, 8-bit block-scaled products, Muon (no counterpart in the reference;
+ * they stand beside kn_multimatmul_grouped, nerf_linear_fm and
+ * nerf_adam_step).
+ * ------------------------------------------------------------------------- */
+enum { NERF_F32 = 0, NERF_BF16 = 1, NERF_F16 = 2 };   /* element types */
+
+/* nerf_route: each row's k of E experts and their weights.
+ *   s = softmax(logits) or sigmoid(logits); key = s + bias (bias NULL: the
+ *   order is that of the logits). groups > 1: E / groups neighbours are a
+ *   group; only the top_groups groups with the highest score (their highest
+ *   key, or with group_top2 the sum of their two highest, from s + bias) stay.
+ *   The k highest keys are chosen, as in exact arithmetic, ties to the lowest
+ *   index; weights = scale * s, with renorm divided by the sum of the chosen s.
+ *   NaN keys count as the lowest; a row that holds a NaN logit (or +inf under
+ *   softmax) gets NaN weights, one whose (chosen) logits are all -inf zeros.
+ *   E <= 1024, k <= 32, groups <= 64.
+ * nerf_route_backward: d logits [T][E] (contiguous, the logits' type) from
+ *   d weights [T][k] and the forward's experts. */
+typedef struct NerfRoute {
+  const void* logits;      /* [T][E], rows ld elements apart */
+  int64_t ld;
+  int64_t T;
+  int type, E, k;
+  int sigmoid, groups, top_groups, group_top2, renorm;
+  const float* bias;       /* [E] or NULL */
+  float scale;
+  float* weights;          /* [T][k] */
+  int* experts;            /* [T][k] */
+} NerfRoute;
+int nerf_route(const NerfRoute* d, nerf_stream_t stream);
+int nerf_route_backward(const NerfRoute* d, const float* dweights, void* dlogits,
+                        nerf_stream_t stream);
+
+/* nerf_expert_plan: the n = T * k slots (t * k + j) sorted by expert, slots of
+ *   one expert in their order. order [n]: slot of each sorted row (-1 behind
+ *   the last expert's); position [n]: sorted row of each slot (-1 where the
+ *   expert is not in [0, E)); offsets [E + 1]. Workspace 16-byte aligned. */
+size_t nerf_expert_plan_workspace(int64_t n, int E);
+int nerf_expert_plan(const int* experts, int64_t n, int E, int* order, int* position, int* offsets,
+                     void* workspace, size_t workspace_bytes, nerf_stream_t stream);
+
+/* nerf_expert_combine: out[t] = sum_j weights[t][j] y[position[t][j]] (y
+ *   [rows][N], out [T][N] of one type, contiguous; positions outside of
+ *   [0, rows) add nothing). _backward: d y [rows][N] (zeros where order is -1)
+ *   and d weights [T][k]; either may be NULL. */
+int nerf_expert_combine(const void* y, int type, int64_t rows, int64_t N, const float* weights,
+                        const int* position, int64_t T, int k, void* out, nerf_stream_t stream);
+int nerf_expert_combine_backward(const void* y, int type, int64_t rows, int64_t N,
+                                 const float* weights, const int* position, const int* order,
+                                 const void* dout, int64_t T, int k, void* dy, float* dweights,
+                                 nerf_stream_t stream);
+
+/* nerf_fp8_linear: out [M][N] = x [M][K] W^T (+ bias, ReLU) with x rounded to
+ *   e4m3 in blocks of 1 x 128 and W given in e4m3 blocks of 128 x 128, each
+ *   block with a power-of-two scale (E8M0: byte b stands for 2^(b - 127), 255
+ *   for NaN): the smallest that brings the block's largest magnitude to 448 or
+ *   less. Sums in FP32, one rounding to out_type.
+ *   wq [E][N][Kp] (Kp = K rounded up to 128, zeros behind K; 16-byte aligned),
+ *   ws [E][ceil(N / 128)][Kp / 128]. offsets NULL: one matrix. offsets [E + 1]:
+ *   rows offsets[e] .. offsets[e + 1] take matrix e; rows behind offsets[E]
+ *   become zeros. order (with slots >= 1): row i is x[order[i] / slots], a row
+ *   of zeros where that is no row of x. bias: [E][N] FP32.
+ * nerf_fp8_quantize_weight: a stack of matrices [E][N][K] (rows ldw, matrices
+ *   stack_stride elements apart) to wq, ws. */
+typedef struct NerfFp8Linear {
+  const void* x;           /* x_rows rows, ldx elements apart (without order: x_rows = M) */
+  int64_t ldx, x_rows;
+  const int* order;        /* [M] or NULL */
+  int x_type, out_type, slots, E, relu;
+  int64_t M, N, K;
+  const void* wq;
+  const void* ws;
+  const int* offsets;      /* [E + 1] or NULL */
+  const float* bias;       /* [E][N] or NULL */
+  void* out;               /* rows ldo elements apart */
+  int64_t ldo;
+} NerfFp8Linear;
+size_t nerf_fp8_linear_workspace(int64_t M, int64_t K, int E, int grouped);
+int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_bytes,
+                    nerf_stream_t stream);
+int nerf_fp8_quantize_weight(const void* w, int type, int64_t stack_stride, int64_t ldw, int E,
+                             int64_t N, int64_t K, void* wq, void* ws, nerf_stream_t stream);
+
+/* nerf_muon: Muon's update of n stacks of matrices (beside nerf_adam_step), or
+ *   (update 0) the orthogonalisation alone, out = NS(g) in g's type.
+ *   buf = momentum buf + g; u = nesterov ? g + momentum buf : buf;
+ *   X = u / (|u| + eps); steps x { A = X X^T; X = a X + (b A + c A A) X } with
+ *   (a, b, c) = (3.4445, -4.7750, 2.0315), on the transpose of a tall matrix;
+ *   out = out (1 - lr weight_decay) - lr sqrt(max(1, m / n)) X.
+ *   clip >= 0: g is clamped to [-clip, clip] on its way in. lr_device (one
+ *   float on the device) goes before lr where it is not NULL. Update: FP32.
+ *   A matrix with a value that is not finite becomes NaN; zeros stay zeros.
+ *   Workspace 16-byte aligned. */
+typedef struct NerfMuonGroup {
+  void* out;               /* [count][m][n], matrices out_stride elements apart */
+  const void* g;           /* [count][m][n], matrices g_stride elements apart */
+  float* momentum;         /* [count][m][n] contiguous; NULL without update */
+  int64_t m, n, count, out_stride, g_stride;
+} NerfMuonGroup;
+typedef struct NerfMuonOptions {
+  int type, update, nesterov, steps;
+  float lr, momentum, weight_decay, eps, clip;
+  const float* lr_device;
+} NerfMuonOptions;
+size_t nerf_muon_workspace(const NerfMuonGroup* groups, int n);
+int nerf_muon(const NerfMuonGroup* groups, int n, const NerfMuonOptions* o, void* workspace,
+              size_t workspace_bytes, nerf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

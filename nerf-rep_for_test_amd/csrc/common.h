@@ -24,7 +24,7 @@ int check_launch(const char* what);
     if (!(cond)) return ::nerfhip::fail(NERF_E_ARG, (msg));      \
   } while (0)
 
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // CU count of the device a stream launches on (persistent grids: one workgroup
 // per CU), cached per device ordinal; races only write the same value. The

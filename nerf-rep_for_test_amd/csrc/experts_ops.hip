@@ -1,0 +1,870 @@
+// Gated experts: the gate that routes each row to k of E experts, the plan that
+// sorts the (row, choice) slots by expert, and the join of the experts' outputs;
+// with the backward passes of gate and join.
+#include "common.h"
+
+namespace nerfhip {
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChoices = 32;
+constexpr int kMaxGroups = 64;
+
+struct RouteArgs {
+  const void* logits;   // [T][E], rows ld apart
+  int64_t ld;
+  int64_t T;
+  int E, k, sigmoid, groups, top_groups, group_top2, renorm;
+  const float* bias;    // [E] or null
+  float scale;
+  float* weights;       // [T][k]
+  int* experts;         // [T][k]
+};
+
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+// Reductions over the L (16 or 64) lanes of a row: inside 16 lanes by DPP.
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int L, class OP>
+__device__ __forceinline__ unsigned reduce32(unsigned v, OP op) {
+  v = op(v, dpp<0xB1>(v));    // lane ^ 1
+  v = op(v, dpp<0x4E>(v));    // lane ^ 2
+  v = op(v, dpp<0x141>(v));   // the other four of 8
+  v = op(v, dpp<0x140>(v));   // the other eight of 16
+  if constexpr (L == 64) {
+    v = op(v, (unsigned)__shfl_xor((int)v, 16));
+    v = op(v, (unsigned)__shfl_xor((int)v, 32));
+  }
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float row_max(float v) {
+  return __uint_as_float(reduce32<L>(__float_as_uint(v), [](unsigned a, unsigned b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+  return __uint_as_float(reduce32<L>(__float_as_uint(v), [](unsigned a, unsigned b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+template <int L>
+__device__ __forceinline__ unsigned row_or(unsigned v) {
+  return reduce32<L>(v, [](unsigned a, unsigned b) { return a | b; });
+}
+template <int L>
+__device__ __forceinline__ double row_sum(double v) {
+  for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d);
+  return v;
+}
+
+// (key, index) with the higher key, or at equal keys the lower index, over the lanes of a row.
+template <int L>
+__device__ __forceinline__ void row_best(float& key, int& idx) {
+  // ordered as unsigned: sign bit flipped, negatives inverted; the index inverted below it
+  const unsigned b = __float_as_uint(key + 0.0f);   // (-0 counts as 0)
+  unsigned hi = b ^ ((unsigned)((int)b >> 31) | 0x80000000u), lo = ~(unsigned)idx;
+  auto step = [&](unsigned h, unsigned l) {
+    const bool other = h > hi || (h == hi && l > lo);
+    hi = other ? h : hi;
+    lo = other ? l : lo;
+  };
+  step(dpp<0xB1>(hi), dpp<0xB1>(lo));
+  step(dpp<0x4E>(hi), dpp<0x4E>(lo));
+  step(dpp<0x141>(hi), dpp<0x141>(lo));
+  step(dpp<0x140>(hi), dpp<0x140>(lo));
+  if constexpr (L == 64) {
+    step((unsigned)__shfl_xor((int)hi, 16), (unsigned)__shfl_xor((int)lo, 16));
+    step((unsigned)__shfl_xor((int)hi, 32), (unsigned)__shfl_xor((int)lo, 32));
+  }
+  key = __uint_as_float(hi & 0x80000000u ? hi ^ 0x80000000u : ~hi);
+  idx = (int)~lo;
+}
+template <int L>
+__device__ __forceinline__ void row_best(double& key, int& idx) {
+  for (int d = 1; d < L; d *= 2) {
+    const double k2 = __shfl_xor(key, d);
+    const int i2 = __shfl_xor(idx, d);
+    if (k2 > key || (k2 == key && i2 < idx)) {
+      key = k2;
+      idx = i2;
+    }
+  }
+}
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+template <class F>
+__device__ __forceinline__ F lowest();
+template <>
+__device__ __forceinline__ float lowest<float>() { return -3.402823466e+38f; }
+template <>
+__device__ __forceinline__ double lowest<double>() { return -1.7976931348623157e+308; }
+
+// An expert's index from a lane's value v: runs of 4 neighbours (one 8- or 16-byte load).
+template <int L>
+__device__ __forceinline__ int expert_of(int lane, int v) {
+  return ((v >> 2) * L + lane) * 4 + (v & 3);
+}
+
+// Chooses a row's k experts (into chosen[], the same in all of its lanes' view of LDS). In 32 bits
+// (F = float) it returns whether the order could be another one in exact arithmetic: two
+// neighbours in the order (or the last kept and first dropped group) nearer than the keys' error
+// and not made of equal inputs. Such rows are done again with F = double, so the choice is that
+// of exact arithmetic while nearly every row pays for 32 bits only. Without a bias the keys are
+// the logits themselves and nothing but groups' sums can be in doubt.
+template <class F, int L, int V, class T>
+__device__ bool choose(const RouteArgs& a, const T* row, const float (&x)[V], float top, float* keys, int* chosen,
+                       int lane) {
+  constexpr bool k32 = sizeof(F) == 4;
+  F key[V];
+  const bool scored = a.bias != nullptr || (a.groups > 1 && a.group_top2);
+  F sum = 0;
+  if (scored) {
+    if (a.sigmoid) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) key[v] = (F)1 / ((F)1 + exp_of(-(F)x[v]));
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        key[v] = expert_of<L>(lane, v) < a.E ? exp_of((F)x[v] - (F)top) : (F)0;
+        sum += key[v];
+      }
+      sum = row_sum<L>(sum);
+#pragma unroll
+      for (int v = 0; v < V; ++v) key[v] = key[v] / sum;
+    }
+    if (a.bias) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int e = expert_of<L>(lane, v);
+        if (e < a.E) key[v] += (F)a.bias[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = (F)x[v];
+  }
+  // NaN and -inf as the lowest number: in order before what is out of reach (-inf)
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    key[v] = key[v] > lowest<F>() ? key[v] : lowest<F>();
+    if (expert_of<L>(lane, v) >= a.E) key[v] = -(F)__builtin_inff();
+  }
+  bool doubt = false;
+  // twice what two keys (or groups' sums of two keys) can be off in 32 bits: the scores (at most 1) by
+  // 1e-6 with the error of the softmax's sum, each addition by half a step
+  auto near = [&](F p, F q) { return p - q < (F)4e-6 + (F)4.8e-7 * (p < 0 ? -p : p); };
+  if (a.groups > 1) {
+    // the row's keys through LDS: lane j < groups takes group j
+    F* ks = (F*)keys;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = expert_of<L>(lane, v);
+      if (e < a.E) ks[e] = key[v];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    const int per = a.E / a.groups;
+    F* gs = ks + a.E;
+    for (int j = lane; j < a.groups; j += L) {
+      F b1 = -(F)__builtin_inff(), b2 = b1;
+      for (int i = 0; i < per; ++i) {
+        const F v = ks[j * per + i];
+        b2 = v > b1 ? b1 : (v > b2 ? v : b2);
+        b1 = v > b1 ? v : b1;
+      }
+      gs[j] = a.group_top2 && per > 1 ? (b1 > lowest<F>() / 2 && b2 > lowest<F>() / 2 ? b1 + b2 : lowest<F>()) : b1;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    unsigned long long keep = 0;
+    F last = __builtin_inff(), first = -(F)__builtin_inff();   // lowest kept, highest dropped
+    for (int j = 0; j < a.groups; ++j) {
+      const F mine = gs[j];
+      int better = 0;
+      for (int i = 0; i < a.groups; ++i) better += gs[i] > mine || (gs[i] == mine && i < j);
+      if (better < a.top_groups) {
+        keep |= 1ull << j;
+        last = mine < last ? mine : last;
+      } else {
+        first = mine > first ? mine : first;
+      }
+    }
+    // (max of logits without a bias: exact)
+    if (k32 && scored && a.top_groups < a.groups && first > lowest<F>() / 2) doubt = near(last, first);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = expert_of<L>(lane, v);
+      if (!a.bias && e < a.E) key[v] = (F)x[v] > lowest<F>() ? (F)x[v] : lowest<F>();   // the order of the logits
+      if (e < a.E && !((keep >> (e / per)) & 1)) key[v] = -(F)__builtin_inff();
+    }
+  }
+  const int rounds = k32 && a.bias && a.k < a.E ? a.k + 1 : a.k;   // one more: the first one left out
+  F before = __builtin_inff();
+  int ib = -1;
+  for (int j = 0; j < rounds; ++j) {
+    F best = -(F)__builtin_inff();
+    int idx = 0x7fffffff;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = expert_of<L>(lane, v);
+      const bool b = key[v] > best || (key[v] == best && e < idx);
+      best = b ? key[v] : best;
+      idx = b ? e : idx;
+    }
+    row_best<L>(best, idx);
+    if (k32 && a.bias && j > 0 && best > lowest<F>() && near(before, best))
+      doubt = doubt || !((float)row[ib] == (float)row[idx] && a.bias[ib] == a.bias[idx]);
+    before = best;
+    ib = idx;
+    if (j < a.k && lane == 0) chosen[j] = idx;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (expert_of<L>(lane, v) == idx) {
+        key[v] = -(F)__builtin_inff();
+      }
+  }
+  return doubt;
+}
+
+// A chosen expert's part in the weights, r_j of the formulas: w_j = scale * r_j.
+// Renormalised: s_j / sum of the chosen s, with the chosen logits' largest taken out first
+// (m: their maximum; for sigmoid s e^-m = 1 / (e^m + e^(m - l)), m <= 0), so that scores too small
+// for 32 bits still have their ratios.
+__device__ __forceinline__ float chosen_part(const RouteArgs& a, float l, float m) {
+  if (a.renorm) return a.sigmoid ? 1.0f / (expf(m) + expf(m - l)) : expf(l - m);
+  return a.sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - m);
+}
+
+// Rows of L lanes, 256 / L rows in a workgroup. Reads the logits once, writes k weights and
+// experts: bound by HBM for large T, by the k rounds of the choice where E is small.
+template <int L, int V, class T, bool VEC>
+__device__ __forceinline__ void load_logits(const T* row, int E, int lane, float (&x)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; v += 4) {
+    const int e = expert_of<L>(lane, v);
+    if (VEC) {
+      if (e < E) {
+        const Vec<T, 4> q = *(const Vec<T, 4>*)(row + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[v + i] = (float)q.v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[v + i] = -__builtin_inff();
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[v + i] = e + i < E ? (float)row[e + i] : -__builtin_inff();
+    }
+  }
+}
+
+template <int L, int V, class T, bool VEC>
+__global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
+  extern __shared__ double route_lds[];
+  constexpr int R = 256 / L;
+  const int lane = threadIdx.x % L, r = threadIdx.x / L;
+  const int64_t t = (int64_t)blockIdx.x * R + r;
+  const int per_row = a.groups > 1 ? a.E + a.groups : 0;
+  float* keys = (float*)(route_lds + (int64_t)r * per_row);
+  int* chosen = (int*)(route_lds + (int64_t)R * per_row) + r * kMaxChoices;
+  // (a workgroup's last rows may lie behind T: they do the last row again and store nothing, so that
+  // a wave's lanes stay together)
+  const int64_t tr = t < a.T ? t : a.T - 1;
+  const T* row = (const T*)a.logits + tr * a.ld;
+  float x[V];
+  load_logits<L, V, T, VEC>(row, a.E, lane, x);
+  float top = -__builtin_inff();
+  unsigned bad = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    top = fmaxf(top, x[v]);
+    bad |= x[v] != x[v];
+  }
+  top = row_max<L>(top);
+  bad = row_or<L>(bad) | (!a.sigmoid && top == __builtin_inff());
+  if (choose<float, L, V>(a, row, x, top, keys, chosen, lane)) choose<double, L, V>(a, row, x, top, keys, chosen, lane);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  float m = -__builtin_inff();
+  if (a.renorm) {
+    for (int j = lane; j < a.k; j += L) m = fmaxf(m, (float)row[chosen[j]]);
+    m = row_max<L>(m);
+    if (a.sigmoid) m = fminf(m, 0.0f);
+  } else {
+    m = top;
+  }
+  float sum = 0.0f;
+  if (a.renorm) {
+    for (int j = lane; j < a.k; j += L) sum += chosen_part(a, (float)row[chosen[j]], m);
+    sum = row_sum<L>(sum);
+  } else if (!a.sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += expert_of<L>(lane, v) < a.E ? expf(x[v] - top) : 0.0f;
+    sum = row_sum<L>(sum);
+  } else {
+    sum = 1.0f;
+  }
+  const bool nothing = m == -__builtin_inff();   // every (chosen) logit is -inf
+  if (t < a.T) {
+    for (int j = lane; j < a.k; j += L) {
+      const int e = chosen[j];
+      float w = nothing ? 0.0f : chosen_part(a, (float)row[e], m) / sum * a.scale;
+      if (bad) w = __builtin_nanf("");
+      a.weights[t * a.k + j] = w;
+      a.experts[t * a.k + j] = e;
+    }
+  }
+}
+
+struct RouteBwdArgs {
+  RouteArgs f;          // logits, sizes, score, scale; experts: the forward's choice
+  const float* dw;      // [T][k]
+  void* dlogits;        // [T][E], contiguous
+};
+
+// d logits of a row: renormalised, only the chosen ones have a gradient:
+//   softmax: scale r_j (g_j - sum_i r_i g_i);  sigmoid: that times (1 - s_j);
+// not renormalised: softmax: p_e (scale g_e - sum_i scale g_i p_i) for every e; sigmoid: scale g s (1 - s).
+// The row is put together in LDS and written in one sweep.
+template <int L, int V, class T, bool VEC>
+__global__ __launch_bounds__(256) void route_backward_kernel(const RouteBwdArgs b) {
+  extern __shared__ float bwd_lds[];
+  const RouteArgs& a = b.f;
+  constexpr int R = 256 / L;
+  const int lane = threadIdx.x % L, r = threadIdx.x / L;
+  const int64_t t = (int64_t)blockIdx.x * R + r, tr = t < a.T ? t : a.T - 1;
+  const T* row = (const T*)a.logits + tr * a.ld;
+  float* buf = bwd_lds + r * V * L;
+  float x[V], top = -__builtin_inff(), sum = 0.0f;
+  unsigned bad = 0;
+  load_logits<L, V, T, VEC>(row, a.E, lane, x);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    top = fmaxf(top, x[v]);
+    bad |= x[v] != x[v];
+  }
+  top = row_max<L>(top);
+  bad = row_or<L>(bad) | (!a.sigmoid && top == __builtin_inff());
+#pragma unroll
+  for (int v = 0; v < V; ++v) buf[expert_of<L>(lane, v)] = 0.0f;
+  const int* ex = a.experts + tr * a.k;
+  const float* dw = b.dw + tr * a.k;
+  float m = top;
+  if (a.renorm) {
+    m = -__builtin_inff();
+    for (int j = lane; j < a.k; j += L) {
+      const int e = ex[j];
+      if (e >= 0 && e < a.E) m = fmaxf(m, (float)row[e]);
+    }
+    m = row_max<L>(m);
+    if (a.sigmoid) m = fminf(m, 0.0f);
+    for (int j = lane; j < a.k; j += L) {
+      const int e = ex[j];
+      if (e >= 0 && e < a.E) sum += chosen_part(a, (float)row[e], m);
+    }
+    sum = row_sum<L>(sum);
+  } else if (!a.sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += expert_of<L>(lane, v) < a.E ? expf(x[v] - top) : 0.0f;
+    sum = row_sum<L>(sum);
+  } else {
+    sum = 1.0f;
+  }
+  const bool nothing = m == -__builtin_inff();
+  float dot = 0.0f;
+  if (a.renorm || !a.sigmoid) {
+    for (int j = lane; j < a.k; j += L) {
+      const int e = ex[j];
+      if (e >= 0 && e < a.E) dot += chosen_part(a, (float)row[e], m) / sum * dw[j];
+    }
+    dot = row_sum<L>(dot);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  for (int j = lane; j < a.k; j += L) {
+    const int e = ex[j];
+    if (e >= 0 && e < a.E) {
+      const float l = (float)row[e], p = chosen_part(a, l, m) / sum;
+      float d;
+      if (a.renorm) {
+        d = p * (dw[j] - dot);
+        if (a.sigmoid) d = d / (1.0f + expf(l));          // 1 - s
+      } else {
+        d = a.sigmoid ? dw[j] * p * (1.0f / (1.0f + expf(l))) : dw[j] * p;
+      }
+      buf[e] = d * a.scale;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  if (t < a.T) {
+    T* out = (T*)b.dlogits + t * a.E;
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      const int e = expert_of<L>(lane, v);
+      Vec<T, 4> o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float d = buf[e + i];
+        if (!a.renorm && !a.sigmoid) d -= a.scale * dot * expf(x[v + i] - top) / sum;
+        if (nothing) d = 0.0f;
+        if (bad) d = __builtin_nanf("");
+        o.v[i] = (T)d;
+      }
+      if (VEC) {
+        if (e < a.E) *(Vec<T, 4>*)(out + e) = o;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (e + i < a.E) out[e + i] = o.v[i];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the plan
+
+// A stable counting sort of the n slots by expert. A wave counts, and later places, a run of
+// neighbouring slots, 64 at a time in order: lanes with the same expert are found by ballots over
+// the bits of its number, so the places follow from counts alone (no atomics that decide an order).
+__device__ __forceinline__ unsigned long long same_expert(int e, bool live, int bits) {
+  unsigned long long peers = __ballot(live);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (e >> b) & 1;
+    const unsigned long long m = __ballot(one);
+    peers &= one ? m : ~m;
+  }
+  return peers;
+}
+
+constexpr int kPlanSegs = 256;    // runs of slots (one wave each) of a large plan
+constexpr int kPlanSmall = 4096;  // up to here one workgroup does everything (LDS: 18 words an expert)
+bool plan_is_small(int64_t n, int E) { return n <= kPlanSmall && E <= 512; }
+
+__device__ __forceinline__ void plan_count(const int* experts, int64_t lo, int64_t hi, int E, int* cnt, int lane, int bits) {
+  for (int64_t i = lo; i < hi; i += 64) {
+    const int e = i + lane < hi ? experts[i + lane] : -1;
+    const bool live = e >= 0 && e < E;
+    const unsigned long long peers = same_expert(e, live, bits);
+    if (live && __builtin_ctzll(peers) == lane) cnt[e] += __builtin_popcountll(peers);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+__device__ __forceinline__ void plan_place(const int* experts, int64_t lo, int64_t hi, int E, int* at, int lane, int bits,
+                                           int* order, int* position) {
+  for (int64_t i = lo; i < hi; i += 64) {
+    const bool in = i + lane < hi;
+    const int e = in ? experts[i + lane] : -1;
+    const bool live = e >= 0 && e < E;
+    const unsigned long long peers = same_expert(e, live, bits);
+    int p = -1;
+    if (live) p = at[e] + __builtin_popcountll(peers & ((1ull << lane) - 1));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    if (live && __builtin_ctzll(peers) == lane) at[e] += __builtin_popcountll(peers);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    if (in) position[i + lane] = p;
+    if (live) order[p] = (int)(i + lane);
+  }
+}
+
+// Exclusive prefix sums of tot[0..E) into base[0..E], by the whole workgroup (a power of two of
+// 256 threads or more; part: one word for each wave).
+__device__ __forceinline__ void prefix(const int* tot, int* base, int E, int* part) {
+  const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, w = t >> 6;
+  const int per = (E + nt - 1) / nt;
+  int mine = 0;
+  for (int i = 0; i < per; ++i) mine += t * per + i < E ? tot[t * per + i] : 0;
+  int sum = mine;
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 63) part[w] = sum;
+  __syncthreads();
+  int off = sum - mine;
+  for (int i = 0; i < w; ++i) off += part[i];
+  for (int i = 0; i < per; ++i) {
+    const int e = t * per + i;
+    if (e < E) {
+      base[e] = off;
+      off += tot[e];
+      if (e == E - 1) base[E] = off;
+    }
+  }
+  __syncthreads();
+}
+
+// One workgroup of 16 waves: counts, prefix sums and places in one launch.
+__global__ __launch_bounds__(1024) void plan_small_kernel(const int* experts, int n, int E, int bits, int* order,
+                                                          int* position, int* offsets) {
+  extern __shared__ int plan_lds[];   // counts [16][E], totals [E], bases [E + 1]
+  __shared__ int part[16];
+  int* cnt = plan_lds;
+  int* tot = cnt + 16 * E;
+  int* base = tot + E;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
+  for (int i = t; i < 16 * E; i += 1024) cnt[i] = 0;
+  __syncthreads();
+  const int seg = ((n + 1023) / 1024) * 64;
+  const int lo = w * seg < n ? w * seg : n, hi = lo + seg < n ? lo + seg : n;
+  plan_count(experts, lo, hi, E, cnt + w * E, lane, bits);
+  __syncthreads();
+  for (int e = t; e < E; e += 1024) {
+    int s = 0;
+    for (int i = 0; i < 16; ++i) {
+      const int c = cnt[i * E + e];
+      cnt[i * E + e] = s;
+      s += c;
+    }
+    tot[e] = s;
+  }
+  __syncthreads();
+  prefix(tot, base, E, part);
+  for (int i = t; i < 16 * E; i += 1024) cnt[i] += base[i % E];
+  for (int e = t; e <= E; e += 1024) offsets[e] = base[e];
+  for (int i = base[E] + t; i < n; i += 1024) order[i] = -1;
+  __syncthreads();
+  plan_place(experts, lo, hi, E, cnt + w * E, lane, bits, order, position);
+}
+
+// counts [E][kPlanSegs]
+__global__ __launch_bounds__(64) void plan_count_kernel(const int* experts, int64_t n, int64_t seg, int E, int bits,
+                                                        int* counts) {
+  extern __shared__ int plan_lds[];
+  const int lane = threadIdx.x;
+  for (int e = lane; e < E; e += 64) plan_lds[e] = 0;
+  __syncthreads();
+  const int64_t lo = blockIdx.x * seg < n ? blockIdx.x * seg : n, hi = lo + seg < n ? lo + seg : n;
+  plan_count(experts, lo, hi, E, plan_lds, lane, bits);
+  __syncthreads();
+  for (int e = lane; e < E; e += 64) counts[(int64_t)e * kPlanSegs + blockIdx.x] = plan_lds[e];
+}
+
+// One wave for each expert: its runs' counts become where they begin; totals [E].
+__global__ __launch_bounds__(64) void plan_scan_kernel(int* counts, int* totals) {
+  int4* row = (int4*)(counts + (int64_t)blockIdx.x * kPlanSegs);
+  const int lane = threadIdx.x;
+  static_assert(kPlanSegs == 256, "4 counts for each of 64 lanes");
+  int4 c = row[lane];
+  const int mine = c.x + c.y + c.z + c.w;
+  int sum = mine;
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 63) totals[blockIdx.x] = sum;
+  sum -= mine;
+  int4 o;
+  o.x = sum;
+  o.y = o.x + c.x;
+  o.z = o.y + c.y;
+  o.w = o.z + c.z;
+  row[lane] = o;
+}
+
+__global__ __launch_bounds__(256) void plan_place_kernel(const int* experts, int64_t n, int64_t seg, int E, int bits,
+                                                         const int* counts, const int* totals, int* order, int* position,
+                                                         int* offsets) {
+  extern __shared__ int plan_lds[];   // bases [E + 1], places [4][E]
+  __shared__ int part[4];
+  int* base = plan_lds;
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
+  int* at = plan_lds + E + 1 + w * E;
+  prefix(totals, base, E, part);
+  const int s = (int)blockIdx.x * 4 + w;
+  for (int e = lane; e < E; e += 64) at[e] = base[e] + counts[(int64_t)e * kPlanSegs + s];
+  if (blockIdx.x == 0)
+    for (int e = t; e <= E; e += 256) offsets[e] = base[e];
+  for (int64_t i = base[E] + (int64_t)blockIdx.x * 256 + t; i < n; i += (int64_t)gridDim.x * 256) order[i] = -1;
+  __syncthreads();
+  const int64_t lo = s * seg < n ? s * seg : n, hi = lo + seg < n ? lo + seg : n;
+  plan_place(experts, lo, hi, E, at, lane, bits, order, position);
+}
+
+// ---------------------------------------------------------------- the join
+
+template <class T, int W>
+__device__ __forceinline__ void load_w(float (&f)[W], const T* p, int64_t room, bool vec) {
+  if (vec) {
+    const Vec<T, W> v = *(const Vec<T, W>*)p;
+#pragma unroll
+    for (int i = 0; i < W; ++i) f[i] = (float)v.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) f[i] = i < room ? (float)p[i] : 0.0f;
+  }
+}
+template <class T, int W>
+__device__ __forceinline__ void store_w(T* p, const float (&f)[W], int64_t room, bool vec) {
+  if (vec) {
+    Vec<T, W> v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.v[i] = (T)f[i];
+    *(Vec<T, W>*)p = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (i < room) p[i] = (T)f[i];
+  }
+}
+
+// out[t] = sum_j w[t][j] y[position[t][j]] in the order of j, in 32 bits. A thread takes 16 bytes
+// of an output row. Bound by HBM.
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, int64_t rows, int64_t N,
+                                                      const float* __restrict__ w, const int* __restrict__ position,
+                                                      int64_t Tn, int k, T* __restrict__ out) {
+  constexpr int W = 16 / sizeof(T);
+  const int64_t cols = cdiv(N, W), total = Tn * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / cols, n = (i - t * cols) * W;
+    float acc[W] = {};
+#pragma unroll 4
+    for (int j = 0; j < k; ++j) {
+      const int p = position[t * k + j];
+      if (p < 0 || p >= rows) continue;
+      const float c = w[t * k + j];
+      float v[W];
+      load_w<T, W>(v, y + p * N + n, N - n, VEC);
+#pragma unroll
+      for (int q = 0; q < W; ++q) acc[q] = __builtin_fmaf(c, v[q], acc[q]);
+    }
+    store_w<T, W>(out + t * N + n, acc, N - n, VEC);
+  }
+}
+
+// d y[position[t][j]] = w[t][j] d out[t], d w[t][j] = d out[t] . y[position[t][j]]: one wave for
+// each t reads d out[t] once; the rows behind the last expert's get zeros.
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restrict__ y, int64_t rows, int64_t N,
+                                                               const float* __restrict__ w, const int* __restrict__ position,
+                                                               const int* __restrict__ order,
+                                                               const T* __restrict__ dout, int64_t Tn, int k,
+                                                               T* __restrict__ dy, float* __restrict__ dw) {
+  constexpr int W = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  const int64_t waves = (int64_t)gridDim.x * 4;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < Tn; t += waves) {
+    for (int j = 0; j < k; ++j) {
+      const int p = position[t * k + j];
+      const bool live = p >= 0 && p < rows;
+      const float c = w[t * k + j];
+      float dot = 0.0f;
+      if (live) {
+        for (int64_t n = lane * W; n < N; n += 64 * W) {
+          float d[W], v[W];
+          load_w<T, W>(d, dout + t * N + n, N - n, VEC);
+          if (dw) {
+            load_w<T, W>(v, y + p * N + n, N - n, VEC);
+#pragma unroll
+            for (int q = 0; q < W; ++q) dot = __builtin_fmaf(d[q], v[q], dot);
+          }
+          if (dy) {
+#pragma unroll
+            for (int q = 0; q < W; ++q) v[q] = c * d[q];
+            store_w<T, W>(dy + p * N + n, v, N - n, VEC);
+          }
+        }
+      }
+      if (dw) {
+        dot = row_sum<64>(dot);
+        if (lane == 0) dw[t * k + j] = dot;
+      }
+    }
+  }
+  if (dy) {
+    for (int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); p < rows; p += waves)
+      if (order[p] < 0)
+        for (int64_t n = lane; n < N; n += 64) dy[p * N + n] = (T)0.0f;
+  }
+}
+
+// ---------------------------------------------------------------- launches
+
+int check_route(const NerfRoute* d, const char* who, bool fwd) {
+  const std::string at(who);
+  if (!d) return fail(NERF_E_ARG, at + ": null pointer");
+  if (!d->logits || !d->experts || (fwd && !d->weights)) return fail(NERF_E_ARG, at + ": null pointer");
+  if (d->T < 1 || d->T >= (1ll << 31) || d->E < 1 || d->E > kMaxExperts || d->ld < 0)
+    return fail(NERF_E_ARG, at + ": bad size (1 to 1024 experts)");
+  if (d->k < 1 || d->k > kMaxChoices || d->k > d->E) return fail(NERF_E_ARG, at + ": k must be 1 to 32, and at most E");
+  if (d->groups < 1 || d->groups > kMaxGroups || d->E % d->groups || d->top_groups < 1 || d->top_groups > d->groups ||
+      (int64_t)d->top_groups * (d->E / d->groups) < d->k)
+    return fail(NERF_E_ARG, at + ": groups must divide E, and top_groups of them hold k experts");
+  if (d->type < NERF_F32 || d->type > NERF_F16) return fail(NERF_E_ARG, at + ": bad type");
+  return 0;
+}
+
+RouteArgs route_args(const NerfRoute* d) {
+  RouteArgs a;
+  a.logits = d->logits;
+  a.ld = d->ld;
+  a.T = d->T;
+  a.E = d->E;
+  a.k = d->k;
+  a.sigmoid = d->sigmoid;
+  a.groups = d->groups;
+  a.top_groups = d->top_groups;
+  a.group_top2 = d->group_top2;
+  a.renorm = d->renorm;
+  a.bias = d->bias;
+  a.scale = d->scale;
+  a.weights = d->weights;
+  a.experts = d->experts;
+  return a;
+}
+
+template <int L, int V, class T, bool VEC>
+void go_route(const RouteArgs& a, const float* dw, void* dlogits, hipStream_t st) {
+  constexpr int R = 256 / L;
+  const dim3 grid((unsigned)cdiv(a.T, R));
+  if (dlogits) {
+    RouteBwdArgs b{a, dw, dlogits};
+    hipLaunchKernelGGL((route_backward_kernel<L, V, T, VEC>), grid, dim3(256), R * V * L * 4, st, b);
+  } else {
+    const size_t lds = (size_t)R * (a.groups > 1 ? a.E + a.groups : 0) * 8 + R * kMaxChoices * 4;
+    hipLaunchKernelGGL((route_kernel<L, V, T, VEC>), grid, dim3(256), lds, st, a);
+  }
+}
+
+template <class T, bool VEC>
+void go_route_e(const RouteArgs& a, const float* dw, void* dl, hipStream_t st) {
+  if (a.E <= 64) go_route<16, 4, T, VEC>(a, dw, dl, st);
+  else if (a.E <= 128) go_route<16, 8, T, VEC>(a, dw, dl, st);
+  else if (a.E <= 256) go_route<16, 16, T, VEC>(a, dw, dl, st);
+  else if (a.E <= 512) go_route<64, 8, T, VEC>(a, dw, dl, st);
+  else go_route<64, 16, T, VEC>(a, dw, dl, st);
+}
+
+template <class T>
+void go_route_t(const RouteArgs& a, const float* dw, void* dl, hipStream_t st) {
+  const bool vec = a.E % 4 == 0 && a.ld % 4 == 0 && (uintptr_t)a.logits % (4 * sizeof(T)) == 0 &&
+                   (uintptr_t)dl % (4 * sizeof(T)) == 0;
+  if (vec) go_route_e<T, true>(a, dw, dl, st);
+  else go_route_e<T, false>(a, dw, dl, st);
+}
+
+int go_route_any(const NerfRoute* d, const float* dw, void* dl, hipStream_t st) {
+  const RouteArgs a = route_args(d);
+  if (d->type == NERF_F32) go_route_t<float>(a, dw, dl, st);
+  else if (d->type == NERF_BF16) go_route_t<bf16>(a, dw, dl, st);
+  else go_route_t<f16>(a, dw, dl, st);
+  return 0;
+}
+
+int bits_of(int E) {
+  int b = 0;
+  while ((1 << b) < E) ++b;
+  return b;
+}
+
+}  // namespace
+}  // namespace nerfhip
+
+using namespace nerfhip;
+
+extern "C" {
+
+int nerf_route(const NerfRoute* d, nerf_stream_t stream) {
+  if (const int rc = check_route(d, "nerf_route", true)) return rc;
+  go_route_any(d, nullptr, nullptr, as_stream(stream));
+  return check_launch("nerf_route");
+}
+
+int nerf_route_backward(const NerfRoute* d, const float* dweights, void* dlogits, nerf_stream_t stream) {
+  if (const int rc = check_route(d, "nerf_route_backward", false)) return rc;
+  NERF_REQUIRE(dweights && dlogits, "nerf_route_backward: null pointer");
+  go_route_any(d, dweights, dlogits, as_stream(stream));
+  return check_launch("nerf_route_backward");
+}
+
+size_t nerf_expert_plan_workspace(int64_t n, int E) {
+  return E < 1 || plan_is_small(n, E) ? 0 : (size_t)E * (kPlanSegs + 1) * 4;
+}
+
+int nerf_expert_plan(const int* experts, int64_t n, int E, int* order, int* position, int* offsets, void* workspace,
+                     size_t workspace_bytes, nerf_stream_t stream) {
+  NERF_REQUIRE(experts && order && position && offsets, "nerf_expert_plan: null pointer");
+  NERF_REQUIRE(n >= 1 && n < (1ll << 31) && E >= 1 && E <= kMaxExperts, "nerf_expert_plan: bad size (1 to 1024 experts)");
+  const hipStream_t st = as_stream(stream);
+  const int bits = bits_of(E);
+  if (plan_is_small(n, E)) {
+    hipLaunchKernelGGL(plan_small_kernel, dim3(1), dim3(1024), (size_t)(18 * E + 1) * 4, st, experts, (int)n, E, bits,
+                       order, position, offsets);
+    return check_launch("nerf_expert_plan");
+  }
+  NERF_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= nerf_expert_plan_workspace(n, E),
+               "nerf_expert_plan: workspace too small or unaligned");
+  int* counts = (int*)workspace;
+  int* totals = counts + (int64_t)E * kPlanSegs;
+  const int64_t seg = cdiv(cdiv(n, kPlanSegs), 64) * 64;
+  hipLaunchKernelGGL(plan_count_kernel, dim3(kPlanSegs), dim3(64), (size_t)E * 4, st, experts, n, seg, E, bits, counts);
+  hipLaunchKernelGGL(plan_scan_kernel, dim3((unsigned)E), dim3(64), 0, st, counts, totals);
+  hipLaunchKernelGGL(plan_place_kernel, dim3(kPlanSegs / 4), dim3(256), (size_t)(5 * E + 1) * 4, st, experts, n, seg, E, bits,
+                     counts, totals, order, position, offsets);
+  return check_launch("nerf_expert_plan");
+}
+
+int nerf_expert_combine(const void* y, int type, int64_t rows, int64_t N, const float* weights, const int* position,
+                        int64_t T, int k, void* out, nerf_stream_t stream) {
+  NERF_REQUIRE(y && weights && position && out, "nerf_expert_combine: null pointer");
+  NERF_REQUIRE(rows >= 1 && N >= 1 && T >= 1 && k >= 1 && type >= NERF_F32 && type <= NERF_F16,
+               "nerf_expert_combine: bad size or type");
+  const hipStream_t st = as_stream(stream);
+  const int size = type == NERF_F32 ? 4 : 2, W = 16 / size;
+  const int64_t blocks = cdiv(T * cdiv(N, W), 256);
+  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536)), block(256);
+  const bool vec = N % W == 0 && ((uintptr_t)y | (uintptr_t)out) % 16 == 0;
+#define NERF_JOIN(TT)                                                                                               \
+  do {                                                                                                              \
+    auto* kern = vec ? combine_kernel<TT, true> : combine_kernel<TT, false>;                                        \
+    hipLaunchKernelGGL(kern, grid, block, 0, st, (const TT*)y, rows, N, weights, position, T, k, (TT*)out);         \
+  } while (0)
+  if (type == NERF_F32) NERF_JOIN(float);
+  else if (type == NERF_BF16) NERF_JOIN(bf16);
+  else NERF_JOIN(f16);
+#undef NERF_JOIN
+  return check_launch("nerf_expert_combine");
+}
+
+int nerf_expert_combine_backward(const void* y, int type, int64_t rows, int64_t N, const float* weights,
+                                 const int* position, const int* order, const void* dout, int64_t T, int k, void* dy,
+                                 float* dweights, nerf_stream_t stream) {
+  NERF_REQUIRE(y && weights && position && order && dout && (dy || dweights), "nerf_expert_combine_backward: null pointer");
+  NERF_REQUIRE(rows >= 1 && N >= 1 && T >= 1 && k >= 1 && type >= NERF_F32 && type <= NERF_F16,
+               "nerf_expert_combine_backward: bad size or type");
+  const hipStream_t st = as_stream(stream);
+  const int W = type == NERF_F32 ? 4 : 8;
+  const int64_t most = T > rows ? T : rows, blocks = cdiv(most, 4);
+  const dim3 grid((unsigned)(blocks < 65536 ? blocks : 65536)), block(256);
+  const bool vec = N % W == 0 && ((uintptr_t)y | (uintptr_t)dout | (uintptr_t)dy) % 16 == 0;
+#define NERF_JOIN(TT)                                                                                              \
+  do {                                                                                                             \
+    auto* kern = vec ? combine_backward_kernel<TT, true> : combine_backward_kernel<TT, false>;                     \
+    hipLaunchKernelGGL(kern, grid, block, 0, st, (const TT*)y, rows, N, weights, position, order, (const TT*)dout, \
+                       T, k, (TT*)dy, dweights);                                                                   \
+  } while (0)
+  if (type == NERF_F32) NERF_JOIN(float);
+  else if (type == NERF_BF16) NERF_JOIN(bf16);
+  else NERF_JOIN(f16);
+#undef NERF_JOIN
+  return check_launch("nerf_expert_combine_backward");
+}
+
+}  // extern "C"

@@ -1,0 +1,539 @@
+// 8-bit block-scaled products: e4m3 values with one power-of-two scale (E8M0)
+// for 1 x 128 of the activations and for 128 x 128 of the weights,
+//   y[m][n] = sum_k x[m][k] w[n][k]  (+ bias[n], ReLU),
+// dense, or with rows sorted by expert and a weight matrix for each expert.
+//
+// A block's scale is the smallest 2^e that brings its largest magnitude to 448
+// (e4m3's largest value) or less. Scaling by a power of two is exact, so a
+// value is rounded once, to e4m3, whatever computes it, and the matrix
+// instruction applies the scales itself (v_mfma_scale_f32_16x16x128: one
+// instruction is one block). Sums are FP32 in the matrix accumulators; the
+// result is rounded once, to the output's type. The 8-bit instruction adds 8
+// neighbouring products at the scale of the largest, with 13 bits below it: off
+// by 1.3e-5 of a product's norm (measured, normal values), far below a 16-bit
+// result's step of 2^-8 or 2^-11. An FP32 result takes the FP16 instruction
+// instead (Fp8Wide: exact products, half the rate).
+#include "tile_product.h"
+
+namespace nerfhip {
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// The biased exponent (E8M0) of a block whose largest |x| has these bits; 255 (NaN:
+// the block's products are NaN) where a value is not finite.
+__device__ __forceinline__ int block_scale(unsigned amax) {
+  if (amax >= 0x7f800000u) return 255;
+  const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (e < -127 ? -127 : e) + 127;
+}
+
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ __forceinline__ int pack4(float a, float b, float c, float d) {
+  int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
+}
+
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+// N values of a row from column k on; zeros from K on. VEC: 16-byte loads (whole
+// pieces lie inside or outside of the row).
+template <class T, int N, bool VEC>
+__device__ __forceinline__ void load_row(float (&f)[N], const T* row, int64_t k, int64_t K) {
+  constexpr int W = 16 / sizeof(T);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+      Vec<T, W> v = {};
+      if (k + i < K) v = *(const Vec<T, W>*)(row + k + i);
+#pragma unroll
+      for (int j = 0; j < W; ++j) f[i + j] = (float)v.v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = k + i < K ? (float)row[k + i] : 0.0f;
+  }
+}
+
+// A row of the activations: row i itself, or where `order` is given the row that
+// slot order[i] (of `div` slots for each row) came from; -1: no row of x (zeros).
+__device__ __forceinline__ int64_t source_row(const int* order, int div, int64_t rows, int64_t i) {
+  if (!order) return i;
+  const int s = order[i];
+  return s < 0 || s / div >= rows ? -1 : s / div;
+}
+
+// Rows of x to e4m3 q [M][KB * 128] and packed scales s [ceil(KB / 4)][M] (the bytes of 4
+// neighbouring blocks of one row in one word). 16 lanes take one block of 128: 8 values
+// each, the largest magnitude by 4 steps inside the 16 lanes. Bound by HBM: every byte
+// is read and written once.
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t ldx, const int* __restrict__ order,
+                                                       int div, int64_t rows, int64_t M, int64_t K, int KB,
+                                                       unsigned char* __restrict__ q,
+                                                       unsigned char* __restrict__ s) {
+  const int l = threadIdx.x & 15;
+  const int64_t blocks = M * KB;
+  for (int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); b < blocks; b += (int64_t)gridDim.x * 16) {
+    const int64_t m = b / KB;
+    const int kb = (int)(b - m * KB);
+    const int64_t src = source_row(order, div, rows, m);
+    float f[8] = {};
+    if (src >= 0) load_row<T, 8, VEC>(f, x + src * ldx, (int64_t)kb * 128 + l * 8, K);
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+    const int sc = block_scale(top), e = 127 - sc;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __builtin_ldexpf(f[i], e);
+    int2 v;
+    v.x = pack4(f[0], f[1], f[2], f[3]);
+    v.y = pack4(f[4], f[5], f[6], f[7]);
+    *(int2*)(q + (m * KB + kb) * 128 + l * 8) = v;
+    if (l == 0) s[((kb >> 2) * M + m) * 4 + (kb & 3)] = (unsigned char)sc;
+  }
+}
+
+// Blocks of 128 x 128 of weights (stack [E][N][K], rows ldw apart, matrices sw apart) to
+// e4m3 q [E][N][KB * 128] and scales [E][NB][KB]. One workgroup for each block.
+template <class T>
+__global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restrict__ w, int64_t sw, int64_t ldw,
+                                                              int64_t N, int64_t K, int NB, int KB,
+                                                              unsigned char* __restrict__ q,
+                                                              unsigned char* __restrict__ s) {
+  const int64_t id = blockIdx.x;
+  const int kb = (int)(id % KB);
+  const int nb = (int)(id / KB % NB);
+  const int64_t e = id / KB / NB;
+  const int t = threadIdx.x, l = t & 15, r0 = t >> 4;
+  const T* base = w + e * sw;
+  float f[8][8];
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t n = (int64_t)nb * 128 + i * 16 + r0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t k = (int64_t)kb * 128 + l * 8 + j;
+      f[i][j] = n < N && k < K ? (float)base[n * ldw + k] : 0.0f;
+      top = max(top, abs_bits(f[i][j]));
+    }
+  }
+  for (int d = 1; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+  __shared__ unsigned part[4];
+  if ((t & 63) == 0) part[t >> 6] = top;
+  __syncthreads();
+  top = max(max(part[0], part[1]), max(part[2], part[3]));
+  const int sc = block_scale(top), ex = 127 - sc;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t n = (int64_t)nb * 128 + i * 16 + r0;
+    if (n < N) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[i][j] = __builtin_ldexpf(f[i][j], ex);
+      int2 v;
+      v.x = pack4(f[i][0], f[i][1], f[i][2], f[i][3]);
+      v.y = pack4(f[i][4], f[i][5], f[i][6], f[i][7]);
+      *(int2*)(q + ((e * N + n) * KB + kb) * 128 + l * 8) = v;
+    }
+  }
+  if (t == 0) s[id] = (unsigned char)sc;
+}
+
+struct LinearArgs {
+  const void* x;              // the activations' rows (skinny form)
+  int64_t ldx, x_rows;
+  const int* order;           // or null
+  int div;
+  const unsigned char* q;     // quantised rows [M][KB * 128] (tiled form)
+  const unsigned* s;          // [ceil(KB / 4)][M]
+  const unsigned char* wq;    // [E][N][KB * 128]
+  const unsigned char* ws;    // [E][NB][KB]
+  const int* offsets;         // [E + 1], or null (dense: E = 1)
+  int E;
+  const float* bias;          // [E][N], or null
+  int relu;
+  int64_t M, N, K;
+  int KB, NB;
+  void* out;                  // [M][N], rows ldo apart
+  int64_t ldo;
+};
+
+// Rows [lo, hi) of expert e; e == E: the rows behind the last expert's (no weights: zeros).
+__device__ __forceinline__ void expert_rows(const LinearArgs& a, int e, int64_t& lo, int64_t& hi) {
+  if (!a.offsets) {
+    lo = 0;
+    hi = a.M;
+    return;
+  }
+  lo = a.offsets[e];
+  hi = e < a.E ? a.offsets[e + 1] : a.M;
+  lo = lo < 0 ? 0 : (lo > a.M ? a.M : lo);
+  hi = hi < lo ? lo : (hi > a.M ? a.M : hi);
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_run(T* at, const float (&v)[N], int64_t room, bool vec) {
+  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  if (vec && room >= N) {
+#pragma unroll
+    for (int i = 0; i < N; i += W) {
+      Vec<T, W> o;
+#pragma unroll
+      for (int j = 0; j < W; ++j) o.v[j] = (T)v[i + j];
+      *(Vec<T, W>*)(at + i) = o;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < room) at[i] = (T)v[i];
+  }
+}
+
+// max(v, 0) that keeps NaN
+__device__ __forceinline__ float relu_of(float v) { return v < 0.0f ? 0.0f : v; }
+
+// ---------------------------------------------------------------- tiled form
+
+// Workgroup -> (expert, row tile): experts' row tiles one after another. Wave 0 sums the
+// experts' tile counts 64 at a time until the tile is met.
+template <int BM>
+__device__ __forceinline__ bool find_tile(const LinearArgs& a, int tile, int& e, int64_t& m0, int64_t& hi) {
+  if (!a.offsets) {
+    e = 0;
+    m0 = (int64_t)tile * BM;
+    hi = a.M;
+    return m0 < a.M;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int base = 0; base <= a.E; base += 64) {
+    const int mine = base + lane;
+    int64_t l = 0, h = 0;
+    if (mine <= a.E) expert_rows(a, mine, l, h);
+    const int n = (int)cdiv(h - l, BM);
+    int sum = n;
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    const unsigned long long met = __ballot(before + sum > tile);
+    if (met) {
+      const int at = __builtin_ctzll(met);
+      e = base + at;
+      const int first = before + __shfl(sum - n, at);
+      expert_rows(a, e, l, h);
+      m0 = l + (int64_t)(tile - first) * BM;
+      hi = h;
+      return true;
+    }
+    before += __shfl(sum, 63);
+  }
+  return false;
+}
+
+template <class S, class T>
+__global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int mtiles, int ntiles) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int64_t id = xcd_tile(blockIdx.x, gridDim.x);
+  const int nt = (int)(id % ntiles), mt = (int)(id / ntiles);
+  int e;
+  int64_t m0, hi;
+  if (!find_tile<S::BM>(a, mt, e, m0, hi)) return;
+  const int64_t n0 = (int64_t)nt * S::BN;
+  TileProduct<S> p;
+  const bool none = e == a.E && a.offsets;
+  const int64_t ld = (int64_t)a.KB * 128;
+  const int eb = none ? 0 : e;
+  p.init((const char*)a.q, ld, m0, hi, (const char*)a.wq + (int64_t)eb * a.N * ld, ld, n0, a.N);
+  if (!none) {
+    const int w = threadIdx.x >> 6;
+    int64_t nb = (n0 + (w % S::WC) * 16 * S::TN) / 128;
+    nb = nb < a.NB ? nb : a.NB - 1;
+    const unsigned char* ws = a.ws + ((int64_t)eb * a.NB + nb) * a.KB;
+    const unsigned* srow[S::TM];
+    unsigned sw[S::TM], sw_next[S::TM];
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i) {
+      const int64_t m = m0 + p.m(i);
+      srow[i] = a.s + (m < hi ? m : hi - 1);
+      sw[i] = sw_next[i] = *srow[i];
+    }
+    int sn = ws[0];
+    p.load(lds);
+    for (int k = 0; k < a.KB; ++k) {
+      stage_ready();
+      typename TileProduct<S>::Frags f;
+      p.read(f, lds + (k & 1) * S::kStage);
+      int sn_next = 0;
+      if (k + 1 < a.KB) {
+        sn_next = ws[k + 1];
+        if ((k & 3) == 3) {
+#pragma unroll
+          for (int i = 0; i < S::TM; ++i) sw_next[i] = *(srow[i] += a.M);
+        }
+        p.load(lds + ((k + 1) & 1) * S::kStage);
+      }
+      int sm[S::TM];
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) sm[i] = (int)sw[i];
+      p.mul(f, sm, sn);
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) sw[i] = (k & 3) == 3 ? sw_next[i] : sw[i] >> 8;
+      sn = sn_next;
+    }
+  }
+  const int64_t n = n0 + p.n();
+  const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) % 16 == 0;
+  float bias[4 * S::TN];
+#pragma unroll
+  for (int c = 0; c < 4 * S::TN; ++c)
+    bias[c] = a.bias && !none && n + c < a.N ? a.bias[(int64_t)eb * a.N + n + c] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < S::TM; ++i) {
+    const int64_t m = m0 + p.m(i);
+    if (m < hi && n < a.N) {
+      float v[4 * S::TN];
+#pragma unroll
+      for (int c = 0; c < 4 * S::TN; ++c) {
+        v[c] = p.acc[i][c / 4][c % 4] + bias[c];
+        if (a.relu) v[c] = relu_of(v[c]);
+      }
+      store_run((T*)a.out + m * a.ldo + n, v, a.N - n, vec);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- skinny form
+
+// Few rows for each weight matrix: bound by the weights' bytes. A workgroup of 8 waves
+// takes 16 weight rows; the waves share the blocks of K between them, read the weights
+// straight into the matrix operands (16 rows x 128 B lines, no LDS) and quantise the
+// activations in registers (a row's block lies in 4 lanes), so one launch reads each
+// weight once. The 8 partial sums are added in wave order.
+template <class T, class O, int RT, bool VEC>
+__global__ __launch_bounds__(512) void skinny_kernel(const LinearArgs a) {
+  constexpr int W = 8;
+  __shared__ float part[W][RT][16][17];
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63, g = lane >> 4, r = lane & 15;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int e = blockIdx.y;
+  int64_t lo, hi;
+  expert_rows(a, e, lo, hi);
+  if (lo >= hi) return;
+  const bool none = a.offsets && e == a.E;
+  const int64_t nrow = n0 + r < a.N ? n0 + r : a.N - 1;
+  const int eb = none ? 0 : e;
+  const unsigned char* wrow = a.wq + ((int64_t)eb * a.N + nrow) * a.KB * 128 + g * 16;
+  const unsigned char* ws = a.ws + ((int64_t)eb * a.NB + n0 / 128) * a.KB;
+  for (int64_t m0 = lo; m0 < hi; m0 += 16 * RT) {
+    f32x4 acc[RT];
+    const T* xrow[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      acc[i] = f32x4(0.0f);
+      const int64_t m = m0 + 16 * i + r;
+      const int64_t src = source_row(a.order, a.div, a.x_rows, m < hi ? m : hi - 1);
+      xrow[i] = src < 0 ? nullptr : (const T*)a.x + src * a.ldx;
+    }
+    if (!none) {
+#pragma unroll 4
+      for (int k = w; k < a.KB; k += W) {
+        const i32x4 w0 = *(const i32x4*)(wrow + (int64_t)k * 128);
+        const i32x4 w1 = *(const i32x4*)(wrow + (int64_t)k * 128 + 64);
+        const int sn = ws[k];
+        const i32x8 wf = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          float f0[16] = {}, f1[16] = {};
+          if (xrow[i]) {
+            load_row<T, 16, VEC>(f0, xrow[i], (int64_t)k * 128 + g * 16, a.K);
+            load_row<T, 16, VEC>(f1, xrow[i], (int64_t)k * 128 + 64 + g * 16, a.K);
+          }
+          unsigned top = 0;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) top = max(top, max(abs_bits(f0[c]), abs_bits(f1[c])));
+          top = max(top, (unsigned)__shfl_xor((int)top, 16));
+          top = max(top, (unsigned)__shfl_xor((int)top, 32));
+          const int sc = block_scale(top), ex = 127 - sc;
+          i32x8 xf;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            xf[c] = pack4(__builtin_ldexpf(f0[4 * c], ex), __builtin_ldexpf(f0[4 * c + 1], ex),
+                          __builtin_ldexpf(f0[4 * c + 2], ex), __builtin_ldexpf(f0[4 * c + 3], ex));
+            xf[4 + c] = pack4(__builtin_ldexpf(f1[4 * c], ex), __builtin_ldexpf(f1[4 * c + 1], ex),
+                              __builtin_ldexpf(f1[4 * c + 2], ex), __builtin_ldexpf(f1[4 * c + 3], ex));
+          }
+          if constexpr (sizeof(O) == 4)
+            acc[i] = wide_block(wf, xf, sn, sc, acc[i]);
+          else
+            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[i], 0, 0, 0, sn, 0, sc);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) part[w][i][r][g * 4 + c] = acc[i][c];   // [row m][column n]
+    __syncthreads();
+    for (int o = t; o < RT * 256; o += 512) {
+      const int i = o >> 8, m = (o >> 4) & 15, c = o & 15;
+      float v = part[0][i][m][c];
+#pragma unroll
+      for (int u = 1; u < W; ++u) v += part[u][i][m][c];
+      const int64_t row = m0 + 16 * i + m, n = n0 + c;
+      if (row < hi && n < a.N) {
+        if (a.bias && !none) v += a.bias[(int64_t)eb * a.N + n];
+        if (a.relu) v = relu_of(v);
+        ((O*)a.out)[row * a.ldo + n] = (O)v;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- launches
+
+bool aligned16(const void* p, int64_t ld, int size) {
+  return (uintptr_t)p % 16 == 0 && (uint64_t)ld * size % 16 == 0;
+}
+
+template <class T>
+void launch_quantize(const NerfFp8Linear* d, int KB, unsigned char* q, unsigned char* s, hipStream_t st) {
+  const int64_t groups = cdiv(d->M * KB, 16);
+  const unsigned grid = (unsigned)(groups < 65536 ? groups : 65536);
+  const bool vec = aligned16(d->x, d->ldx, sizeof(T)) && d->K % (16 / sizeof(T)) == 0;
+  auto* kern = vec ? quantize_kernel<T, true> : quantize_kernel<T, false>;
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, st, (const T*)d->x, d->ldx, d->order, d->order ? d->slots : 1,
+                     d->x_rows, d->M, d->K, KB, q, s);
+}
+
+template <class S, class T>
+void launch_product(const LinearArgs& a, hipStream_t st) {
+  const int64_t mt = a.offsets ? a.M / S::BM + a.E + 1 : cdiv(a.M, S::BM), nt = cdiv(a.N, S::BN);
+  hipLaunchKernelGGL((product_kernel<S, T>), dim3((unsigned)(mt * nt)), dim3(S::NT), 2 * S::kStage, st, a, (int)mt,
+                     (int)nt);
+}
+
+template <class T, class O, int RT>
+void launch_skinny(const LinearArgs& a, hipStream_t st) {
+  const bool vec = aligned16(a.x, a.ldx, sizeof(T)) && a.K % 16 == 0;
+  auto* kern = vec ? skinny_kernel<T, O, RT, true> : skinny_kernel<T, O, RT, false>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(a.N, 16), (unsigned)(a.offsets ? a.E + 1 : 1)), dim3(512), 0, st, a);
+}
+
+template <class T>
+void launch_skinny_out(const LinearArgs& a, int out_type, hipStream_t st) {
+  if (out_type == NERF_F32) launch_skinny<T, float, 1>(a, st);
+  else if (out_type == NERF_BF16) launch_skinny<T, bf16, 1>(a, st);
+  else launch_skinny<T, f16, 1>(a, st);
+}
+
+// Few rows for each weight matrix (16, one matrix operand): the skinny form.
+bool is_skinny(int64_t M, int E, bool grouped) { return grouped ? M <= 16 * (int64_t)E : M <= 16; }
+
+int check(const NerfFp8Linear* d) {
+  NERF_REQUIRE(d && d->x && d->wq && d->ws && d->out, "nerf_fp8_linear: null pointer");
+  NERF_REQUIRE(d->M >= 1 && d->N >= 1 && d->K >= 1 && d->M < (1ll << 31) && d->N < (1ll << 31) && d->K < (1ll << 31) - 128,
+               "nerf_fp8_linear: bad size");
+  NERF_REQUIRE(d->x_type >= NERF_F32 && d->x_type <= NERF_F16 && d->out_type >= NERF_F32 && d->out_type <= NERF_F16,
+               "nerf_fp8_linear: bad type");
+  NERF_REQUIRE(d->E >= 1 && d->E <= 65534 && (d->offsets || d->E == 1), "nerf_fp8_linear: E matrices need offsets");
+  NERF_REQUIRE(d->order ? d->slots >= 1 && d->x_rows >= 1 : d->x_rows == d->M, "nerf_fp8_linear: slots or rows of x");
+  NERF_REQUIRE(d->ldx >= 0 && d->ldo >= d->N, "nerf_fp8_linear: row pitch");
+  NERF_REQUIRE((uintptr_t)d->wq % 16 == 0, "nerf_fp8_linear: weights need 16-byte alignment");
+  return 0;
+}
+
+}  // namespace
+}  // namespace nerfhip
+
+using namespace nerfhip;
+
+extern "C" {
+
+size_t nerf_fp8_linear_workspace(int64_t M, int64_t K, int E, int grouped) {
+  if (M < 1 || K < 1 || is_skinny(M, E, grouped != 0)) return 0;
+  const int64_t KB = cdiv(K, 128);
+  return (size_t)(M * KB * 128 + cdiv(KB, 4) * M * 4);
+}
+
+int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_bytes, nerf_stream_t stream) {
+  if (const int rc = check(d)) return rc;
+  const hipStream_t st = as_stream(stream);
+  LinearArgs a;
+  a.x = d->x;
+  a.ldx = d->ldx;
+  a.x_rows = d->x_rows;
+  a.order = d->order;
+  a.div = d->order ? d->slots : 1;
+  a.wq = (const unsigned char*)d->wq;
+  a.ws = (const unsigned char*)d->ws;
+  a.offsets = d->offsets;
+  a.E = d->E;
+  a.bias = d->bias;
+  a.relu = d->relu;
+  a.M = d->M;
+  a.N = d->N;
+  a.K = d->K;
+  a.KB = (int)cdiv(d->K, 128);
+  a.NB = (int)cdiv(d->N, 128);
+  a.out = d->out;
+  a.ldo = d->ldo;
+  a.q = nullptr;
+  a.s = nullptr;
+  if (is_skinny(d->M, d->E, d->offsets != nullptr)) {
+    if (d->x_type == NERF_F32) launch_skinny_out<float>(a, d->out_type, st);
+    else if (d->x_type == NERF_BF16) launch_skinny_out<bf16>(a, d->out_type, st);
+    else launch_skinny_out<f16>(a, d->out_type, st);
+    return check_launch("nerf_fp8_linear");
+  }
+  NERF_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
+                   workspace_bytes >= nerf_fp8_linear_workspace(d->M, d->K, d->E, d->offsets != nullptr),
+               "nerf_fp8_linear: workspace too small or unaligned");
+  unsigned char* q = (unsigned char*)workspace;
+  unsigned char* s = q + d->M * a.KB * 128;
+  a.q = q;
+  a.s = (const unsigned*)s;
+  using S = TileShape<Fp8, 4, 4, 2, 2>;
+  using SW = TileShape<Fp8Wide, 4, 4, 2, 2>;
+  NERF_REQUIRE((d->M / S::BM + d->E + 1) * cdiv(d->N, S::BN) < (1ll << 31), "nerf_fp8_linear: too many tiles");
+  if (d->x_type == NERF_F32) launch_quantize<float>(d, a.KB, q, s, st);
+  else if (d->x_type == NERF_BF16) launch_quantize<bf16>(d, a.KB, q, s, st);
+  else launch_quantize<f16>(d, a.KB, q, s, st);
+  if (const int rc = check_launch("nerf_fp8_linear")) return rc;
+  if (d->out_type == NERF_F32) launch_product<SW, float>(a, st);
+  else if (d->out_type == NERF_BF16) launch_product<S, bf16>(a, st);
+  else launch_product<S, f16>(a, st);
+  return check_launch("nerf_fp8_linear");
+}
+
+int nerf_fp8_quantize_weight(const void* w, int type, int64_t stack_stride, int64_t ldw, int E, int64_t N, int64_t K,
+                             void* q, void* scale, nerf_stream_t stream) {
+  NERF_REQUIRE(w && q && scale, "nerf_fp8_quantize_weight: null pointer");
+  NERF_REQUIRE(E >= 1 && N >= 1 && K >= 1 && type >= NERF_F32 && type <= NERF_F16,
+               "nerf_fp8_quantize_weight: bad size or type");
+  const int64_t KB = cdiv(K, 128), NB = cdiv(N, 128);
+  NERF_REQUIRE(KB < (1ll << 24) && NB < (1ll << 24) && E * NB * KB < (1ll << 31),
+               "nerf_fp8_quantize_weight: too many blocks");
+  NERF_REQUIRE((uintptr_t)q % 8 == 0, "nerf_fp8_quantize_weight: q needs 8-byte alignment");
+  const dim3 grid((unsigned)(E * NB * KB)), block(256);
+  const hipStream_t st = as_stream(stream);
+#define NERF_QW(T)                                                                                          \
+  hipLaunchKernelGGL(quantize_weight_kernel<T>, grid, block, 0, st, (const T*)w, stack_stride, ldw, N, K,   \
+                     (int)NB, (int)KB, (unsigned char*)q, (unsigned char*)scale)
+  if (type == NERF_F32) NERF_QW(float);
+  else if (type == NERF_BF16) NERF_QW(bf16);
+  else NERF_QW(f16);
+#undef NERF_QW
+  return check_launch("nerf_fp8_quantize_weight");
+}
+
+}  // extern "C"

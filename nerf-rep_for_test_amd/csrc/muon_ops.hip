@@ -1,0 +1,456 @@
+// Muon's update: momentum, Newton-Schulz orthogonalisation, weight decay and the step.
+//   buf = mu buf + g,  u = g + mu buf (Nesterov; else u = buf),  X = u / (|u| + eps),
+//   steps times:  A = X X^T,  B = b A + c A A,  X = a X + B X,
+//   p = p (1 - lr wd) - lr sqrt(max(1, m / n)) X;
+// or X alone (orthogonalisation). X is worked on with its short side r as rows ([r][c],
+// the transpose of a tall matrix). The quintic a s + b s^3 + c s^5 keeps singular values
+// within [0, 1.21] (its maximum on [0, 1.21] is 1.2024), which bounds every entry:
+// |X| <= 1.21, |A| <= 1.45, |B| <= 2.81.
+//
+// Products are FP32-accurate on the FP16 matrix cores (tile_product.h, Split): operands
+// as hi + lo FP16, x = hi + lo to 22 bits, three terms in FP32 accumulators. The bounds
+// above let X be held times S (a power of two near sqrt(r c), at most 2^15), A times 2^15
+// and B times 2^14, so lo parts stay clear of FP16's least numbers and nothing overflows.
+// The three products of a step are one launch each over all matrices. A and B are
+// symmetric: only tiles on and below the diagonal are computed and each is stored twice.
+// All sums have a fixed order. X is kept in both layouts (rows for A, its transpose for
+// B X), since the product takes both operands with the reduction axis contiguous.
+#include "tile_product.h"
+
+namespace nerfhip {
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
+constexpr float kScaleA = 32768.0f, kScaleB = 16384.0f;
+constexpr int kMaxGroups = 16;    // stacks of equal matrices in one launch
+constexpr int kNormBlocks = 256;  // partial sums of one matrix's norm, at most
+
+struct Group {
+  void* out;           // parameters (FP32) or results, [count] matrices out_stride apart
+  const void* g;       // [count][m][n], g_stride apart
+  float* buf;          // momentum, contiguous, or null
+  int64_t out_stride, g_stride;
+  char* work;          // per matrix: Xs, Xt, Xt', A, B (split rows)
+  double* norm;        // [count][kNormBlocks]
+  int m, n, r, c, count;
+  int norm_blocks;
+  float s;             // X's scale
+  float adjust;        // sqrt(max(1, m / n))
+};
+
+struct Batch {
+  Group g[kMaxGroups];
+  int end[kMaxGroups];   // prefix sums of the groups' workgroups
+  int count;
+  float mu, clip, eps, decay, lr;
+  const float* lr_dev;
+  int nesterov, type;
+};
+
+// Bytes of a row of `n` values as split chunks.
+__host__ __device__ inline int64_t row_bytes(int n) { return cdiv(n, 32) * 128; }
+
+struct Work {   // one matrix's buffers
+  char *xs, *xt0, *xt1, *a, *b;
+};
+__host__ __device__ inline int64_t work_bytes(int r, int c) {
+  return r * row_bytes(c) + 2 * (int64_t)c * row_bytes(r) + 2 * (int64_t)r * row_bytes(r);
+}
+__device__ __forceinline__ Work work_of(const Group& g, int i) {
+  Work w;
+  w.xs = g.work + i * work_bytes(g.r, g.c);
+  w.xt0 = w.xs + g.r * row_bytes(g.c);
+  w.xt1 = w.xt0 + g.c * row_bytes(g.r);
+  w.a = w.xt1 + g.c * row_bytes(g.r);
+  w.b = w.a + g.r * row_bytes(g.r);
+  return w;
+}
+
+__device__ __forceinline__ int find_group(const Batch& b, int& blk) {
+  int k = 0;
+  while (k + 1 < b.count && blk >= b.end[k]) ++k;
+  blk -= k ? b.end[k - 1] : 0;
+  return k;
+}
+
+struct HiLo {
+  f16 hi, lo;
+};
+__device__ __forceinline__ HiLo split(float v) {
+  HiLo s;
+  s.hi = (f16)v;
+  s.lo = (f16)(v - (float)s.hi);
+  return s;
+}
+
+__device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
+  if (type == NERF_F32) return ((const float*)p)[i];
+  if (type == NERF_BF16) return (float)((const bf16*)p)[i];
+  return (float)((const f16*)p)[i];
+}
+
+__device__ __forceinline__ float clipped(float g, float clip) {   // (NaN stays)
+  if (clip < 0.0f) return g;
+  return g > clip ? clip : (g < -clip ? -clip : g);
+}
+
+// The momentum is advanced and the matrices' squares are summed (64 bits: no overflow, a fixed
+// order).
+__global__ __launch_bounds__(256) void muon_norm_kernel(const Batch b) {
+  int blk = blockIdx.x;
+  const Group& g = b.g[find_group(b, blk)];
+  const int i = blk / g.norm_blocks, part = blk - i * g.norm_blocks;
+  const int64_t n = (int64_t)g.m * g.n;
+  const char* src = (const char*)g.g + i * g.g_stride * (b.type == NERF_F32 ? 4 : 2);
+  float* buf = g.buf ? g.buf + i * n : nullptr;
+  double sum = 0.0;
+  for (int64_t k = (int64_t)part * 256 + threadIdx.x; k < n; k += (int64_t)g.norm_blocks * 256) {
+    float v = clipped(load_any(src, b.type, k), b.clip);
+    if (buf) {
+      const float m = buf[k] * b.mu + v;
+      buf[k] = m;
+      v = b.nesterov ? v + b.mu * m : m;
+    }
+    sum += (double)v * v;
+  }
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  __shared__ double w[4];
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) g.norm[(int64_t)i * kNormBlocks + part] = (w[0] + w[1]) + (w[2] + w[3]);
+}
+
+__device__ __forceinline__ void put8(char* row, int k, const HiLo (&v)[8]) {   // columns k .. k + 8 of a split row
+  f16x8 h, l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    h[i] = v[i].hi;
+    l[i] = v[i].lo;
+  }
+  char* at = row + (k >> 5) * 128 + (k & 31) * 2;
+  *(f16x8*)at = h;
+  *(f16x8*)(at + 64) = l;
+}
+
+// u / (|u| + eps) times S in both layouts. A workgroup takes 64 x 64 of [m][n].
+__global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
+  __shared__ float tile[64][65];
+  __shared__ double wsum[4];
+  int blk = blockIdx.x;
+  const Group& g = b.g[find_group(b, blk)];
+  const int tn = (g.n + 63) / 64, tm = (g.m + 63) / 64;
+  const int i = blk / (tm * tn), t = blk - i * tm * tn, m0 = t / tn * 64, n0 = t % tn * 64;
+  double sum = threadIdx.x < g.norm_blocks ? g.norm[(int64_t)i * kNormBlocks + threadIdx.x] : 0.0;
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  const float inv = (float)((double)g.s / (__builtin_sqrt((wsum[0] + wsum[1]) + (wsum[2] + wsum[3])) + (double)b.eps));
+  const int64_t size = (int64_t)g.m * g.n;
+  const char* src = (const char*)g.g + i * g.g_stride * (b.type == NERF_F32 ? 4 : 2);
+  const float* buf = g.buf ? g.buf + i * size : nullptr;
+  for (int q = threadIdx.x; q < 4096; q += 256) {
+    const int y = q >> 6, x = q & 63;
+    float v = 0.0f;
+    if (m0 + y < g.m && n0 + x < g.n) {
+      const int64_t k = (int64_t)(m0 + y) * g.n + n0 + x;
+      v = clipped(load_any(src, b.type, k), b.clip);
+      if (buf) v = b.nesterov ? v + b.mu * buf[k] : buf[k];
+      v *= inv;
+    }
+    tile[y][x] = v;
+  }
+  __syncthreads();
+  const Work w = work_of(g, i);
+  const bool tall = g.m > g.n;
+  char* mat = tall ? w.xt0 : w.xs;   // rows like [m][n]
+  char* tra = tall ? w.xs : w.xt0;   // rows like [n][m]
+  const int64_t lm = row_bytes(g.n), ln = row_bytes(g.m);
+  const int pn = (g.n + 31) & ~31, pm = (g.m + 31) & ~31;
+  for (int q = threadIdx.x; q < 512; q += 256) {
+    const int row = q >> 3, k = (q & 7) * 8;
+    HiLo v[8];
+    if (m0 + row < g.m && n0 + k < pn) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = split(tile[row][k + e]);
+      put8(mat + (m0 + row) * lm, n0 + k, v);
+    }
+    if (n0 + row < g.n && m0 + k < pm) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = split(tile[k + e][row]);
+      put8(tra + (n0 + row) * ln, m0 + k, v);
+    }
+  }
+}
+
+enum { kStepA = 0, kStepB = 1, kStepX = 2, kStepLast = 3 };
+
+// One product of a step for every matrix of the batch. FLIP: which of the two transposes is read.
+template <class S, int STEP, class T>
+__global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int flip) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  constexpr int TM = S::TM, TN = S::TN;
+  int blk = blockIdx.x;
+  const Group& g = bt.g[find_group(bt, blk)];
+  const int rows = g.r, cols = STEP >= kStepX ? g.c : g.r;
+  const int tm = (rows + S::BM - 1) / S::BM, tn = (cols + S::BN - 1) / S::BN;
+  const int tiles = STEP >= kStepX ? tm * tn : tm * (tm + 1) / 2;
+  const int i = blk / tiles, t = blk - i * tiles;
+  int mt, nt;
+  if (STEP >= kStepX) {
+    mt = t % tm;
+    nt = t / tm;
+  } else {   // the tiles on and below the diagonal, row by row
+    mt = (int)((__builtin_sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+    while (mt * (mt + 1) / 2 > t) --mt;
+    while ((mt + 1) * (mt + 2) / 2 <= t) ++mt;
+    nt = t - mt * (mt + 1) / 2;
+  }
+  const Work w = work_of(g, i);
+  const char* xt = flip ? w.xt1 : w.xt0;
+  const char* M = STEP == kStepA ? w.xs : (STEP == kStepB ? w.a : w.b);
+  const char* N = STEP == kStepA ? w.xs : (STEP == kStepB ? w.a : xt);
+  const int kdim = STEP == kStepA ? g.c : g.r;
+  const int64_t ld = row_bytes(kdim);
+  const int m0 = mt * S::BM, n0 = nt * S::BN, steps = (kdim + 31) / 32;
+  TileProduct<S> p;
+  p.init(M, ld, m0, rows, N, ld, n0, cols);
+  p.load(lds);
+  for (int k = 0; k < steps; ++k) {
+    stage_ready();
+    typename TileProduct<S>::Frags f;
+    p.read(f, lds + (k & 1) * S::kStage);
+    if (k + 1 < steps) p.load(lds + ((k + 1) & 1) * S::kStage);
+    p.mul(f);
+  }
+  // this lane's rows m, columns n .. n + 4 TN
+  const int n = n0 + p.n();
+  char* to = STEP == kStepA ? w.a : (STEP == kStepB ? w.b : w.xs);
+  const char* add = STEP == kStepB ? w.a : w.xs;   // the term beside the product
+  const int64_t lto = row_bytes(cols);
+  constexpr int P = S::BM + 4;   // LDS row of the transposed tile, words
+  unsigned* tr = (unsigned*)lds;
+  __syncthreads();
+  const float unscale = STEP == kStepA ? kScaleA / (g.s * g.s) : 1.0f;
+  const float lr = STEP == kStepLast ? (bt.lr_dev ? *bt.lr_dev : bt.lr) : 0.0f;
+  const bool tall = g.m > g.n;
+#pragma unroll
+  for (int q = 0; q < TM; ++q) {
+    const int ml = p.m(q), m = m0 + ml;
+#pragma unroll
+    for (int h = 0; h < 4 * TN; h += 8) {
+      HiLo v[8];
+      float f[8];
+      const int nn = n + h;
+      f16x8 ah = {}, al = {};
+      if (STEP != kStepA && m < rows && nn < cols) {
+        const char* at = add + m * lto + (nn >> 5) * 128 + (nn & 31) * 2;
+        ah = *(const f16x8*)at;
+        al = *(const f16x8*)(at + 64);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float acc = p.acc[q][(h + e) / 4][(h + e) % 4];
+        float x = acc;
+        const float beside = (float)ah[e] + (float)al[e];
+        if (STEP == kStepA) x = acc * unscale;
+        if (STEP == kStepB) x = kB * (kScaleB / kScaleA) * beside + kC * (kScaleB / (kScaleA * kScaleA)) * acc;
+        if (STEP >= kStepX) x = kA * beside + acc * (1.0f / kScaleB);
+        f[e] = nn + e < cols ? x : 0.0f;
+        if (STEP != kStepLast) v[e] = split(f[e]);
+      }
+      if (STEP == kStepLast) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= 1.0f / g.s;
+        if (tall) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) tr[(p.n() + h + e) * P + ml] = __float_as_uint(f[e]);
+        } else if (m < rows) {
+          T* at = (T*)g.out + i * g.out_stride + (int64_t)m * g.n + nn;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (nn + e < cols) {
+              if (g.buf) at[e] = (T)((float)at[e] * (1.0f - lr * bt.decay) - f[e] * (lr * g.adjust));
+              else at[e] = (T)f[e];
+            }
+        }
+      } else {
+        if (m < rows && nn < ((cols + 31) & ~31)) put8(to + m * lto, nn, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          tr[(p.n() + h + e) * P + ml] =
+              (unsigned)__builtin_bit_cast(unsigned short, v[e].hi) | (unsigned)__builtin_bit_cast(unsigned short, v[e].lo) << 16;
+      }
+    }
+  }
+  if (STEP < kStepX && mt == nt) return;
+  if (STEP == kStepLast && !tall) return;
+  __syncthreads();
+  // the transposed tile: rows n, 8 columns m at a time
+  char* tt = STEP == kStepA ? w.a : (STEP == kStepB ? w.b : (flip ? w.xt0 : w.xt1));
+  const int64_t ltt = row_bytes(rows);
+  for (int q = threadIdx.x; q < S::BN * S::BM / 8; q += S::NT) {
+    const int nl = q / (S::BM / 8), k = q % (S::BM / 8) * 8, nn = n0 + nl, m = m0 + k;
+    if (nn >= cols || m >= ((rows + 31) & ~31)) continue;
+    const unsigned* at = tr + nl * P + k;
+    if (STEP == kStepLast) {
+      T* o = (T*)g.out + i * g.out_stride + (int64_t)nn * g.n + m;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (m + e < rows) {
+          const float x = __uint_as_float(at[e]);
+          if (g.buf) o[e] = (T)((float)o[e] * (1.0f - lr * bt.decay) - x * (lr * g.adjust));
+          else o[e] = (T)x;
+        }
+    } else {
+      HiLo v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned u = m + e < rows ? at[e] : 0u;
+        v[e].hi = __builtin_bit_cast(f16, (unsigned short)(u & 0xffffu));
+        v[e].lo = __builtin_bit_cast(f16, (unsigned short)(u >> 16));
+      }
+      put8(tt + nn * ltt, m, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- launches
+
+int check_group(const NerfMuonGroup& g, bool update) {
+  NERF_REQUIRE(g.out && g.g && (!update || g.momentum), "nerf_muon: null pointer");
+  NERF_REQUIRE(g.m >= 1 && g.n >= 1 && g.count >= 1 && g.m <= (1 << 20) && g.n <= (1 << 20) &&
+                   g.count < (1 << 20) && g.g_stride >= 0 && g.out_stride >= 0,
+               "nerf_muon: bad size");
+  return 0;
+}
+
+int64_t group_bytes(const NerfMuonGroup& g) {
+  const int r = (int)(g.m < g.n ? g.m : g.n), c = (int)(g.m < g.n ? g.n : g.m);
+  return g.count * (work_bytes(r, c) + (int64_t)kNormBlocks * 8);
+}
+
+int64_t count_tiles(const Group& g, int bm, int bn, bool square) {
+  const int64_t tm = cdiv(g.r, bm), tn = cdiv(g.c, bn);
+  return g.count * (square ? tm * (tm + 1) / 2 : tm * tn);
+}
+
+template <class S>
+constexpr size_t lds_bytes() {
+  const size_t a = 2 * S::kStage, b = (size_t)S::BN * (S::BM + 4) * 4;
+  return a > b ? a : b;
+}
+
+template <class S, int STEP, class T>
+int launch_step(Batch& b, int flip, hipStream_t st) {
+  int64_t end = 0;
+  for (int k = 0; k < b.count; ++k) {
+    end += count_tiles(b.g[k], S::BM, S::BN, STEP < kStepX);
+    NERF_REQUIRE(end < (1ll << 31), "nerf_muon: too many tiles");
+    b.end[k] = (int)end;
+  }
+  hipLaunchKernelGGL((muon_product_kernel<S, STEP, T>), dim3((unsigned)end), dim3(S::NT), lds_bytes<S>(), st, b, flip);
+  return check_launch("nerf_muon");
+}
+
+template <class S>
+int run_steps(Batch& b, int steps, bool update, hipStream_t st) {
+  for (int k = 0; k < steps; ++k) {
+    const int flip = k & 1;
+    if (const int rc = launch_step<S, kStepA, float>(b, flip, st)) return rc;
+    if (const int rc = launch_step<S, kStepB, float>(b, flip, st)) return rc;
+    int rc;
+    if (k + 1 < steps) rc = launch_step<S, kStepX, float>(b, flip, st);
+    else if (update || b.type == NERF_F32) rc = launch_step<S, kStepLast, float>(b, flip, st);
+    else if (b.type == NERF_BF16) rc = launch_step<S, kStepLast, bf16>(b, flip, st);
+    else rc = launch_step<S, kStepLast, f16>(b, flip, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace nerfhip
+
+using namespace nerfhip;
+
+extern "C" {
+
+size_t nerf_muon_workspace(const NerfMuonGroup* groups, int n) {
+  size_t s = 0;
+  for (int k = 0; groups && k < n; ++k) s += (size_t)group_bytes(groups[k]);
+  return s;
+}
+
+int nerf_muon(const NerfMuonGroup* groups, int n, const NerfMuonOptions* o, void* workspace, size_t workspace_bytes,
+              nerf_stream_t stream) {
+  NERF_REQUIRE(groups && o, "nerf_muon: null pointer");
+  NERF_REQUIRE(n >= 1 && o->steps >= 1 && o->type >= NERF_F32 && o->type <= NERF_F16 &&
+                   (!o->update || o->type == NERF_F32),
+               "nerf_muon: bad count, steps or type");
+  for (int k = 0; k < n; ++k)
+    if (const int rc = check_group(groups[k], o->update != 0)) return rc;
+  NERF_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= nerf_muon_workspace(groups, n),
+               "nerf_muon: workspace too small or unaligned");
+  const hipStream_t st = as_stream(stream);
+  char* at = (char*)workspace;
+  for (int first = 0; first < n; first += kMaxGroups) {
+    Batch b;
+    b.count = n - first < kMaxGroups ? n - first : kMaxGroups;
+    b.mu = o->momentum;
+    b.clip = o->clip;
+    b.eps = o->eps;
+    b.decay = o->weight_decay;
+    b.lr = o->lr;
+    b.lr_dev = o->lr_device;
+    b.nesterov = o->nesterov;
+    b.type = o->type;
+    int64_t end = 0, split_end[kMaxGroups], tiles64 = 0, tiles = 0;
+    for (int k = 0; k < b.count; ++k) {
+      const NerfMuonGroup& s = groups[first + k];
+      Group& g = b.g[k];
+      g.out = s.out;
+      g.g = s.g;
+      g.buf = o->update ? s.momentum : nullptr;
+      g.out_stride = s.out_stride;
+      g.g_stride = s.g_stride;
+      g.m = (int)s.m;
+      g.n = (int)s.n;
+      g.count = (int)s.count;
+      g.r = g.m < g.n ? g.m : g.n;
+      g.c = g.m < g.n ? g.n : g.m;
+      const int64_t size = s.m * s.n;
+      const int64_t nb = cdiv(size, 2048);
+      g.norm_blocks = (int)(nb < kNormBlocks ? nb : kNormBlocks);
+      int e = 0;
+      while (e < 15 && (1ll << (2 * e)) < size) ++e;
+      g.s = (float)(1 << e);
+      g.adjust = s.m > s.n ? (float)__builtin_sqrt((double)s.m / (double)s.n) : 1.0f;
+      g.norm = (double*)at;
+      at += g.count * (int64_t)kNormBlocks * 8;
+      g.work = at;
+      at += g.count * work_bytes(g.r, g.c);
+      end += (int64_t)g.count * g.norm_blocks;
+      b.end[k] = (int)end;
+      tiles += g.count * cdiv(s.m, 64) * cdiv(s.n, 64);
+      split_end[k] = tiles;
+      tiles64 += count_tiles(g, 128, 128, false);
+      NERF_REQUIRE(end < (1ll << 31) && tiles < (1ll << 31), "nerf_muon: too many tiles");
+    }
+    hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)end), dim3(256), 0, st, b);
+    for (int k = 0; k < b.count; ++k) b.end[k] = (int)split_end[k];
+    hipLaunchKernelGGL(muon_split_kernel, dim3((unsigned)tiles), dim3(256), 0, st, b);
+    if (const int rc = check_launch("nerf_muon")) return rc;
+    // 128 x 128 tiles read each operand half as often; 64 x 64 ones fill the CUs where there are few
+    using Large = TileShape<Split, 4, 4, 2, 2>;
+    using Small = TileShape<Split, 2, 2, 2, 2>;
+    const int rc = tiles64 >= 256 ? run_steps<Large>(b, o->steps, o->update != 0, st)
+                                  : run_steps<Small>(b, o->steps, o->update != 0, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+}  // extern "C"

@@ -93,6 +93,18 @@ SIGNATURES = {
     "kn_multi_row_sum_reduction": (_I, [_P, _I64, _P, _I, _P, _S]),
     "kn_multimatmul_A_transposed": (_I, [_P, _I64, _P, _I64, _P, _I, _P, _S]),
     "kn_render_to_screen": (_I, []),
+    "nerf_route": (_I, [_P, _S]),
+    "nerf_route_backward": (_I, [_P, _P, _P, _S]),
+    "nerf_expert_plan_workspace": (_SZ, [_I64, _I]),
+    "nerf_expert_plan": (_I, [_P, _I64, _I, _P, _P, _P, _P, _SZ, _S]),
+    "nerf_expert_combine": (_I, [_P, _I, _I64, _I64, _P, _P, _I64, _I, _P, _S]),
+    "nerf_expert_combine_backward": (_I, [_P, _I, _I64, _I64, _P, _P, _P, _P, _I64, _I, _P, _P,
+                                          _S]),
+    "nerf_muon_workspace": (_SZ, [_P, _I]),
+    "nerf_muon": (_I, [_P, _I, _P, _P, _SZ, _S]),
+    "nerf_fp8_linear_workspace": (_SZ, [_I64, _I64, _I, _I]),
+    "nerf_fp8_linear": (_I, [_P, _P, _SZ, _S]),
+    "nerf_fp8_quantize_weight": (_I, [_P, _I, _I64, _I64, _I, _I64, _I64, _P, _P, _S]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,122 @@
+"""Muon: matrices' updates orthogonalised by Newton-Schulz products
+(csrc/muon_ops.hip), beside nerfhip.adam's Adam.
+
+``orthogonalize`` is the operator alone, ``muon_update`` one step of momentum,
+orthogonalisation, weight decay and step for a list of matrices (17 launches for
+all of them, at most 16 shapes or stacks a set), ``HipMuon`` the optimizer that
+the trainer takes: matrices of hidden layers by Muon, everything else by Adam.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import call, ptr
+from .adam import HipAdam
+from .fp8 import TYPES, on_device_of
+
+STEPS, EPS = 5, 1e-7
+
+
+class _Group(ctypes.Structure):
+    """NerfMuonGroup (include/nerfhip.h)."""
+    _fields_ = [("out", ctypes.c_void_p), ("g", ctypes.c_void_p), ("momentum", ctypes.c_void_p),
+                ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("count", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("g_stride", ctypes.c_int64)]
+
+
+class _Options(ctypes.Structure):
+    """NerfMuonOptions (include/nerfhip.h)."""
+    _fields_ = [("type", ctypes.c_int), ("update", ctypes.c_int), ("nesterov", ctypes.c_int),
+                ("steps", ctypes.c_int), ("lr", ctypes.c_float), ("momentum", ctypes.c_float),
+                ("weight_decay", ctypes.c_float), ("eps", ctypes.c_float), ("clip", ctypes.c_float),
+                ("lr_device", ctypes.c_void_p)]
+
+
+def _run(groups, options, like):
+    arr = (_Group * len(groups))(*groups)
+    need = _lib.lib().nerf_muon_workspace(ctypes.addressof(arr), len(groups))
+    with on_device_of(like):
+        ws = torch.empty((need,), device=like.device, dtype=torch.uint8)
+        call("nerf_muon", ctypes.addressof(arr), len(groups), ctypes.addressof(options), ptr(ws), need,
+             _lib.stream_of(like.device))
+
+
+def _check_steps(steps):
+    if int(steps) != steps or not 1 <= steps <= 100:
+        raise ValueError("muon: steps must be a whole number from 1 to 100")
+    return int(steps)
+
+
+@torch.no_grad()
+def orthogonalize(g, steps=STEPS, eps=EPS):
+    """Newton-Schulz orthogonalisation of a matrix [m, n] or a stack [.., m, n] (float32, bfloat16, float16;
+    result in the same type): X = g / (|g| + eps), then ``steps`` times X = a X + (b A + c A A) X with
+    A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315); singular values end near 1. Sums, norms and products hold
+    float32 accuracy whatever the type. A matrix with a value that is not finite becomes NaN. No gradient."""
+    if g.dim() < 2 or g.dtype not in TYPES:
+        raise ValueError("orthogonalize: g must be [.., m, n] float32, bfloat16 or float16")
+    steps = _check_steps(steps)
+    if not 0.0 < eps < float("inf"):
+        raise ValueError("orthogonalize: eps must be positive")
+    m, n = g.shape[-2:]
+    if max(m, n) > 1 << 20:
+        raise ValueError("orthogonalize: sides up to 2^20")
+    _lib.require_gpu(g)
+    g = g.contiguous()
+    out = torch.empty_like(g)
+    if out.numel() == 0:
+        return out
+    o = _Options(TYPES[g.dtype], 0, 0, steps, 0.0, 0.0, 0.0, float(eps), -1.0, None)
+    _run([_Group(ptr(out), ptr(g), None, m, n, out.numel() // (m * n), m * n, m * n)], o, g)
+    return out
+
+
+def _float32_matrix(t, shape, what):
+    if t.dtype != torch.float32 or t.dim() != 2 or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise ValueError(f"muon_update: {what} must be contiguous float32 matrices of their parameter's shape")
+
+
+@torch.no_grad()
+def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=STEPS, eps=EPS,
+                clip=None):
+    """One Muon step for a list of matrices, in place (params and momenta):
+    buf = momentum * buf + g; u = g + momentum * buf (``nesterov``; else buf);
+    p = p * (1 - lr * weight_decay) - lr * sqrt(max(1, m / n)) * orthogonalize(u).
+    ``lr``: a number, or one float32 on the device (then the step can be captured and replayed with another
+    one). ``clip``: gradients clamped to [-clip, clip] on their way in (the gradients themselves stay)."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError("muon_update: params, grads and momenta must be lists of one length")
+    steps = _check_steps(steps)
+    if not 0.0 <= momentum < 1.0 or not 0.0 < eps < float("inf") or not 0.0 <= weight_decay < float("inf"):
+        raise ValueError("muon_update: momentum must be in [0, 1), eps positive, weight_decay >= 0")
+    if clip is not None and not clip >= 0:
+        raise ValueError("muon_update: clip must be None or >= 0")
+    seen, groups = set(), []
+    for p, g, b in zip(params, grads, momenta):
+        _float32_matrix(p, None, "params")
+        _float32_matrix(g, p.shape, "grads")
+        _float32_matrix(b, p.shape, "momenta")
+        if p.device != params[0].device or g.device != p.device or b.device != p.device:
+            raise ValueError("muon_update: all tensors must be on one device")
+        if max(p.shape) > 1 << 20:
+            raise ValueError("muon_update: sides up to 2^20")
+        if p.numel() == 0:
+            continue
+        for t in (p, b):
+            if t.data_ptr() in seen:
+                raise ValueError("muon_update: a matrix (or momentum) is there twice")
+            seen.add(t.data_ptr())
+        groups.append(_Group(ptr(p), ptr(g), ptr(b), *p.shape, 1, 0, 0))
+    dev_lr = torch.is_tensor(lr)
+    if dev_lr and (lr.dtype != torch.float32 or lr.numel() != 1 or (params and lr.device != params[0].device)):
+        raise ValueError("muon_update: a tensor lr must be one float32 on the parameters' device")
+    if not groups:
+        return
+    _lib.require_gpu(params[0])
+    o = _Options(0, 1, int(bool(nesterov)), steps, 0.0 if dev_lr else float(lr), float(momentum), float(weight_decay),
+                 float(eps), -1.0 if clip is None else float(clip), ptr(lr) if dev_lr else None)
+    _run(groups, o, params[0])
