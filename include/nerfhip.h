@@ -678,7 +678,7 @@ typedef struct NerfFp8Linear {
   void* out;               /* rows ldo elements apart */
   int64_t ldo;
 } NerfFp8Linear;
-size_t nerf_fp8_linear_workspace(int64_t M, int64_t K, int E, int grouped);
+size_t nerf_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int E, int grouped);
 int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_bytes,
                     nerf_stream_t stream);
 int nerf_fp8_quantize_weight(const void* w, int type, int64_t stack_stride, int64_t ldw, int E,

@@ -36,6 +36,14 @@ __device__ __forceinline__ int pack4(float a, float b, float c, float d) {
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
 }
 
+// The largest value of 16 neighbouring lanes, by DPP.
+__device__ __forceinline__ unsigned max16(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));    // lane ^ 1
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));    // lane ^ 2
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));   // the other four of 8
+  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+}
+
 template <class T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
@@ -57,6 +65,24 @@ __device__ __forceinline__ void load_row(float (&f)[N], const T* row, int64_t k,
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) f[i] = k + i < K ? (float)row[k + i] : 0.0f;
+  }
+}
+
+// 8 values of a row from column k on as they are; zeros from K on.
+template <class T, bool VEC>
+__device__ __forceinline__ void load_raw(T (&v)[8], const T* row, int64_t k, int64_t K) {
+  constexpr int W = 16 / sizeof(T);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < 8; i += W) {
+      Vec<T, W> q = {};
+      if (k + i < K) q = *(const Vec<T, W>*)(row + k + i);
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i + j] = q.v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? row[k + i] : (T)0.0f;
   }
 }
 
@@ -88,8 +114,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
     unsigned top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+    top = max16(top);
     const int sc = block_scale(top), e = 127 - sc;
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = __builtin_ldexpf(f[i], e);
@@ -239,63 +264,19 @@ __device__ __forceinline__ bool find_tile(const LinearArgs& a, int tile, int& e,
   return false;
 }
 
+// This lane's columns' bias (zeros without).
+template <class S>
+__device__ __forceinline__ void load_bias(const LinearArgs& a, int64_t e, int64_t n, float (&bias)[4 * S::TN]) {
+#pragma unroll
+  for (int c = 0; c < 4 * S::TN; ++c) bias[c] = a.bias && n + c < a.N ? a.bias[e * a.N + n + c] : 0.0f;
+}
+
+// The tile's results: bias, ReLU, one rounding, rows below hi.
 template <class S, class T>
-__global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int mtiles, int ntiles) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int64_t id = xcd_tile(blockIdx.x, gridDim.x);
-  const int nt = (int)(id % ntiles), mt = (int)(id / ntiles);
-  int e;
-  int64_t m0, hi;
-  if (!find_tile<S::BM>(a, mt, e, m0, hi)) return;
-  const int64_t n0 = (int64_t)nt * S::BN;
-  TileProduct<S> p;
-  const bool none = e == a.E && a.offsets;
-  const int64_t ld = (int64_t)a.KB * 128;
-  const int eb = none ? 0 : e;
-  p.init((const char*)a.q, ld, m0, hi, (const char*)a.wq + (int64_t)eb * a.N * ld, ld, n0, a.N);
-  if (!none) {
-    const int w = threadIdx.x >> 6;
-    int64_t nb = (n0 + (w % S::WC) * 16 * S::TN) / 128;
-    nb = nb < a.NB ? nb : a.NB - 1;
-    const unsigned char* ws = a.ws + ((int64_t)eb * a.NB + nb) * a.KB;
-    const unsigned* srow[S::TM];
-    unsigned sw[S::TM], sw_next[S::TM];
-#pragma unroll
-    for (int i = 0; i < S::TM; ++i) {
-      const int64_t m = m0 + p.m(i);
-      srow[i] = a.s + (m < hi ? m : hi - 1);
-      sw[i] = sw_next[i] = *srow[i];
-    }
-    int sn = ws[0];
-    p.load(lds);
-    for (int k = 0; k < a.KB; ++k) {
-      stage_ready();
-      typename TileProduct<S>::Frags f;
-      p.read(f, lds + (k & 1) * S::kStage);
-      int sn_next = 0;
-      if (k + 1 < a.KB) {
-        sn_next = ws[k + 1];
-        if ((k & 3) == 3) {
-#pragma unroll
-          for (int i = 0; i < S::TM; ++i) sw_next[i] = *(srow[i] += a.M);
-        }
-        p.load(lds + ((k + 1) & 1) * S::kStage);
-      }
-      int sm[S::TM];
-#pragma unroll
-      for (int i = 0; i < S::TM; ++i) sm[i] = (int)sw[i];
-      p.mul(f, sm, sn);
-#pragma unroll
-      for (int i = 0; i < S::TM; ++i) sw[i] = (k & 3) == 3 ? sw_next[i] : sw[i] >> 8;
-      sn = sn_next;
-    }
-  }
+__device__ __forceinline__ void store_tile(const LinearArgs& a, const TileProduct<S>& p, const float (&bias)[4 * S::TN],
+                                           int64_t m0, int64_t hi, int64_t n0) {
   const int64_t n = n0 + p.n();
   const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) % 16 == 0;
-  float bias[4 * S::TN];
-#pragma unroll
-  for (int c = 0; c < 4 * S::TN; ++c)
-    bias[c] = a.bias && !none && n + c < a.N ? a.bias[(int64_t)eb * a.N + n + c] : 0.0f;
 #pragma unroll
   for (int i = 0; i < S::TM; ++i) {
     const int64_t m = m0 + p.m(i);
@@ -308,6 +289,168 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
       }
       store_run((T*)a.out + m * a.ldo + n, v, a.N - n, vec);
     }
+  }
+}
+
+constexpr int kScaleRun = 512;   // blocks of K whose weights' scales are in LDS at a time
+
+// A stage with its rows' scale words, two of them, and the weights' scale bytes.
+template <class S>
+struct ProductLds {
+  static constexpr int kAll = S::kStage + S::BM * 4;
+  static constexpr size_t kBytes = 2 * kAll + (S::BN / 128 > 0 ? S::BN / 128 : 1) * kScaleRun;
+};
+
+template <class S, class T>
+__global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int mtiles, int ntiles) {
+  using L = ProductLds<S>;
+  static_assert(S::BN % 128 == 0 && 128 % (16 * S::TN) == 0 && S::BM % 64 == 0, "one scale for a wave's columns");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int64_t id = xcd_tile(blockIdx.x, gridDim.x);
+  int e, mt, nt;
+  band_tile(id, mtiles, ntiles, 8, mt, nt);
+  int64_t m0, hi;
+  if (!find_tile<S::BM>(a, mt, e, m0, hi)) return;
+  const int64_t n0 = (int64_t)nt * S::BN;
+  TileProduct<S> p;
+  const bool none = e == a.E && a.offsets;
+  const int64_t ld = (int64_t)a.KB * 128;
+  const int eb = none ? 0 : e;
+  p.init((const char*)a.q, ld, m0, hi, (const char*)a.wq + (int64_t)eb * a.N * ld, ld, n0, a.N);
+  if (!none) {
+    // Scales reach the loop through LDS only, so nothing in it waits for a load into registers:
+    // the rows' words (4 blocks) with each stage, the weights' bytes kScaleRun blocks at a time.
+    const int t = threadIdx.x, w = t >> 6;
+    const unsigned char* ws = a.ws + (int64_t)eb * a.NB * a.KB;
+    const int64_t nb0 = n0 / 128;
+    const unsigned* s0 = (const unsigned*)uniform((int64_t)(a.s + m0));
+    const int rows = (int)(hi - 1 - m0 < S::BM ? hi - 1 - m0 : S::BM);
+    char* bytes = lds + 2 * L::kAll;
+    const unsigned char* mine = (const unsigned char*)bytes + ((w % S::WC) * 16 * S::TN / 128) * kScaleRun;
+    auto load = [&](int k, bool live) {
+      char* stage = lds + (k & 1) * L::kAll;
+      p.load(stage, k, live);
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(s0 + (int64_t)(k >> 2) * a.M), 0, range_of(live),
+                                                        0x00020000);
+#pragma unroll
+      for (int i = 0; i * S::NT < S::BM; ++i) {
+        const int u = __builtin_amdgcn_readfirstlane(w) * 64 + i * S::NT, r = i * S::NT + t;
+        if (u < S::BM)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(
+              rs, (__attribute__((address_space(3))) void*)(stage + S::kStage + u * 4), 4, (r < rows ? r : rows) * 4, 0,
+              0, 0);
+      }
+    };
+    load(0, true);
+    for (int k = 0; k < a.KB; ++k) {
+      if (k % kScaleRun == 0) {
+        if (k) __syncthreads();
+        for (int q = t; q < S::BN / 128 * kScaleRun; q += S::NT) {
+          const int64_t nb = nb0 + q / kScaleRun;
+          const int kb = k + q % kScaleRun;
+          if (kb < a.KB && nb < a.NB) bytes[q] = (char)ws[nb * a.KB + kb];
+        }
+      }
+      stage_ready();
+      const char* stage = lds + (k & 1) * L::kAll;
+      typename TileProduct<S>::Frags f;
+      int sm[S::TM];
+      const int sn = mine[k % kScaleRun];
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) sm[i] = (int)(((const unsigned*)(stage + S::kStage))[p.m(i)] >> (8 * (k & 3)));
+      p.read(f, stage);
+      load(k + 1, k + 1 < a.KB);
+      p.mul(f, sm, sn);
+    }
+    stage_ready();
+  }
+  float bias[4 * S::TN] = {};
+  if (!none) load_bias<S>(a, eb, n0 + p.n(), bias);
+  store_tile<S, T>(a, p, bias, m0, hi, n0);
+}
+
+// ---------------------------------------------------------------- resident form
+
+// Many rows through one small matrix (N <= 256, K <= 256: the width of the framework's networks): bound
+// by reading x and writing y. One workgroup on each CU holds the 8-bit weights in LDS and walks over
+// tiles of 128 rows: the next tile's rows are on their way into registers while this one's products run
+// and its results are stored; a tile is rounded to 8 bits straight into LDS (two buffers, one barrier
+// for each tile), so the activations' 8-bit form never goes to memory.
+constexpr int kResident = 256;
+
+template <class S>
+constexpr size_t resident_lds(int KB) {
+  return (size_t)KB * (S::BN * 128 + 2 * S::BM * 129) + 4 * KB;
+}
+
+template <class S, class X, class T, int KB, bool VEC>
+__global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int mtiles) {
+  static_assert(S::BN == kResident, "all columns in one tile");
+  constexpr int IT = S::BM * KB * 16 / S::NT;   // blocks of 128 for each 16 lanes
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int t = threadIdx.x, w = t >> 6, l = t & 15;
+  const int64_t ld = KB * 128;
+  const char* W = (const char*)a.wq;
+  char* rows = lds + KB * S::BN * 128;                                      // [2][KB][BM][128]
+  unsigned char* sx = (unsigned char*)rows + 2 * KB * S::BM * 128;          // [2][KB][BM]
+  TileProduct<S> p;
+  p.init(W, ld, 0, 1, W, ld, 0, a.N);
+  for (int k = 0; k < KB; ++k) p.load_n(lds + k * S::BN * 128, k, true);
+  int sn[KB];
+  float bias[4 * S::TN];
+  const int nb = (w % S::WC) * 16 * S::TN / 128;
+#pragma unroll
+  for (int k = 0; k < KB; ++k) sn[k] = a.ws[(nb < a.NB ? nb : a.NB - 1) * KB + k];
+  load_bias<S>(a, 0, p.n(), bias);
+  X x[IT][8];
+  auto fetch = [&](int64_t tile) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int b = i * (S::NT / 16) + (t >> 4), r = b % S::BM, kb = b / S::BM;
+      const int64_t m = tile * S::BM + r;
+      load_raw<X, VEC>(x[i], (const X*)a.x + (m < a.M ? m : a.M - 1) * a.ldx, kb * 128 + l * 8, a.K);
+    }
+  };
+  int64_t tile = blockIdx.x;
+  fetch(tile);
+  for (int at = 0; tile < mtiles; tile += gridDim.x, at ^= 1) {
+    char* mine = rows + at * KB * S::BM * 128;
+    unsigned char* smine = sx + at * KB * S::BM;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int b = i * (S::NT / 16) + (t >> 4), r = b % S::BM, kb = b / S::BM;
+      float f[8];
+      unsigned top = 0;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        f[c] = (float)x[i][c];
+        top = max(top, abs_bits(f[c]));
+      }
+      top = max16(top);
+      const int sc = block_scale(top), ex = 127 - sc;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) f[c] = __builtin_ldexpf(f[c], ex);
+      int2 v;
+      v.x = pack4(f[0], f[1], f[2], f[3]);
+      v.y = pack4(f[4], f[5], f[6], f[7]);
+      *(int2*)(mine + kb * S::BM * 128 + r * 128 + (((l >> 1) ^ swz<S::TM>(r)) << 4) + (l & 1) * 8) = v;
+      if (l == 0) smine[kb * S::BM + r] = (unsigned char)sc;
+    }
+    const int64_t next = tile + gridDim.x;
+    if (at == 0 && tile == blockIdx.x) stage_ready();   // (the weights, too)
+    else __syncthreads();
+    fetch(next < mtiles ? next : tile);
+    p.clear();
+#pragma unroll 1   // (the fragments of one block at a time)
+    for (int k = 0; k < KB; ++k) {
+      typename TileProduct<S>::Frags f;
+      int sm[S::TM];
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) sm[i] = smine[k * S::BM + p.m(i)];
+      p.read(f, mine + k * S::BM * 128, lds + k * S::BN * 128);
+      p.mul(f, sm, KB == 1 || k == 0 ? sn[0] : sn[KB - 1]);
+    }
+    store_tile<S, T>(a, p, bias, tile * S::BM, a.M, 0);
   }
 }
 
@@ -418,8 +561,30 @@ void launch_quantize(const NerfFp8Linear* d, int KB, unsigned char* q, unsigned 
 template <class S, class T>
 void launch_product(const LinearArgs& a, hipStream_t st) {
   const int64_t mt = a.offsets ? a.M / S::BM + a.E + 1 : cdiv(a.M, S::BM), nt = cdiv(a.N, S::BN);
-  hipLaunchKernelGGL((product_kernel<S, T>), dim3((unsigned)(mt * nt)), dim3(S::NT), 2 * S::kStage, st, a, (int)mt,
-                     (int)nt);
+  hipLaunchKernelGGL((product_kernel<S, T>), dim3((unsigned)(mt * nt)), dim3(S::NT), ProductLds<S>::kBytes, st, a,
+                     (int)mt, (int)nt);
+}
+
+template <class S, class X, class T, int KB>
+void launch_resident(const LinearArgs& a, hipStream_t st) {
+  const int64_t mt = cdiv(a.M, S::BM), cus = stream_cu_count(st);
+  const bool vec = aligned16(a.x, a.ldx, sizeof(X)) && a.K % (16 / sizeof(X)) == 0;
+  auto* kern = vec ? resident_kernel<S, X, T, KB, true> : resident_kernel<S, X, T, KB, false>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(mt < cus ? mt : cus)), dim3(S::NT), resident_lds<S>(KB), st, a, (int)mt);
+}
+
+template <class X, class T>
+void launch_resident_k(const LinearArgs& a, hipStream_t st) {
+  using S = TileShape<typename std::conditional<sizeof(T) == 4, Fp8Wide, Fp8>::type, 4, 4, 2, 4>;
+  if (a.KB == 1) launch_resident<S, X, T, 1>(a, st);
+  else launch_resident<S, X, T, 2>(a, st);
+}
+
+template <class X>
+void launch_resident_out(const LinearArgs& a, int out_type, hipStream_t st) {
+  if (out_type == NERF_F32) launch_resident_k<X, float>(a, st);
+  else if (out_type == NERF_BF16) launch_resident_k<X, bf16>(a, st);
+  else launch_resident_k<X, f16>(a, st);
 }
 
 template <class T, class O, int RT>
@@ -439,14 +604,20 @@ void launch_skinny_out(const LinearArgs& a, int out_type, hipStream_t st) {
 // Few rows for each weight matrix (16, one matrix operand): the skinny form.
 bool is_skinny(int64_t M, int E, bool grouped) { return grouped ? M <= 16 * (int64_t)E : M <= 16; }
 
+// Many rows through one small matrix: the resident form (a tile for every CU at least).
+bool is_resident(int64_t M, int64_t N, int64_t K, bool grouped) {
+  return !grouped && N <= kResident && K <= kResident && M >= 256 * 128;
+}
+
 int check(const NerfFp8Linear* d) {
   NERF_REQUIRE(d && d->x && d->wq && d->ws && d->out, "nerf_fp8_linear: null pointer");
-  NERF_REQUIRE(d->M >= 1 && d->N >= 1 && d->K >= 1 && d->M < (1ll << 31) && d->N < (1ll << 31) && d->K < (1ll << 31) - 128,
+  NERF_REQUIRE(d->M >= 1 && d->N >= 1 && d->K >= 1 && d->M < (1ll << 31) && d->N < (1ll << 31) && d->K <= (1ll << 23),
                "nerf_fp8_linear: bad size");
   NERF_REQUIRE(d->x_type >= NERF_F32 && d->x_type <= NERF_F16 && d->out_type >= NERF_F32 && d->out_type <= NERF_F16,
                "nerf_fp8_linear: bad type");
   NERF_REQUIRE(d->E >= 1 && d->E <= 65534 && (d->offsets || d->E == 1), "nerf_fp8_linear: E matrices need offsets");
   NERF_REQUIRE(d->order ? d->slots >= 1 && d->x_rows >= 1 : d->x_rows == d->M, "nerf_fp8_linear: slots or rows of x");
+  NERF_REQUIRE(d->offsets || !d->order, "nerf_fp8_linear: order without offsets");
   NERF_REQUIRE(d->ldx >= 0 && d->ldo >= d->N, "nerf_fp8_linear: row pitch");
   NERF_REQUIRE((uintptr_t)d->wq % 16 == 0, "nerf_fp8_linear: weights need 16-byte alignment");
   return 0;
@@ -459,8 +630,8 @@ using namespace nerfhip;
 
 extern "C" {
 
-size_t nerf_fp8_linear_workspace(int64_t M, int64_t K, int E, int grouped) {
-  if (M < 1 || K < 1 || is_skinny(M, E, grouped != 0)) return 0;
+size_t nerf_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int E, int grouped) {
+  if (M < 1 || N < 1 || K < 1 || is_skinny(M, E, grouped != 0) || is_resident(M, N, K, grouped != 0)) return 0;
   const int64_t KB = cdiv(K, 128);
   return (size_t)(M * KB * 128 + cdiv(KB, 4) * M * 4);
 }
@@ -495,8 +666,14 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
     else launch_skinny_out<f16>(a, d->out_type, st);
     return check_launch("nerf_fp8_linear");
   }
+  if (is_resident(d->M, d->N, d->K, d->offsets != nullptr)) {
+    if (d->x_type == NERF_F32) launch_resident_out<float>(a, d->out_type, st);
+    else if (d->x_type == NERF_BF16) launch_resident_out<bf16>(a, d->out_type, st);
+    else launch_resident_out<f16>(a, d->out_type, st);
+    return check_launch("nerf_fp8_linear");
+  }
   NERF_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
-                   workspace_bytes >= nerf_fp8_linear_workspace(d->M, d->K, d->E, d->offsets != nullptr),
+                   workspace_bytes >= nerf_fp8_linear_workspace(d->M, d->N, d->K, d->E, d->offsets != nullptr),
                "nerf_fp8_linear: workspace too small or unaligned");
   unsigned char* q = (unsigned char*)workspace;
   unsigned char* s = q + d->M * a.KB * 128;
@@ -504,14 +681,19 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   a.s = (const unsigned*)s;
   using S = TileShape<Fp8, 4, 4, 2, 2>;
   using SW = TileShape<Fp8Wide, 4, 4, 2, 2>;
+  // 256 x 256 (128 x 128 for a wave, the whole register file) reads half as much LDS for each product,
+  // but one workgroup on a CU has nobody to cover its start and end: for long rows and many tiles
+  // (8192 x 8192 x 8192: 534 us against 591; 32768 rows of 2048 over 32 experts: 269 against 243).
+  using SL = TileShape<Fp8, 8, 8, 2, 2>;
+  const bool large = d->K >= 4096 && cdiv(d->M, 256) * cdiv(d->N, 256) >= 512;
   NERF_REQUIRE((d->M / S::BM + d->E + 1) * cdiv(d->N, S::BN) < (1ll << 31), "nerf_fp8_linear: too many tiles");
   if (d->x_type == NERF_F32) launch_quantize<float>(d, a.KB, q, s, st);
   else if (d->x_type == NERF_BF16) launch_quantize<bf16>(d, a.KB, q, s, st);
   else launch_quantize<f16>(d, a.KB, q, s, st);
   if (const int rc = check_launch("nerf_fp8_linear")) return rc;
   if (d->out_type == NERF_F32) launch_product<SW, float>(a, st);
-  else if (d->out_type == NERF_BF16) launch_product<S, bf16>(a, st);
-  else launch_product<S, f16>(a, st);
+  else if (d->out_type == NERF_BF16) large ? launch_product<SL, bf16>(a, st) : launch_product<S, bf16>(a, st);
+  else large ? launch_product<SL, f16>(a, st) : launch_product<S, f16>(a, st);
   return check_launch("nerf_fp8_linear");
 }
 

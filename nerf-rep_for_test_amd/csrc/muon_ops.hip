@@ -217,12 +217,12 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
   const int m0 = mt * S::BM, n0 = nt * S::BN, steps = (kdim + 31) / 32;
   TileProduct<S> p;
   p.init(M, ld, m0, rows, N, ld, n0, cols);
-  p.load(lds);
+  p.load(lds, 0, true);
   for (int k = 0; k < steps; ++k) {
     stage_ready();
     typename TileProduct<S>::Frags f;
     p.read(f, lds + (k & 1) * S::kStage);
-    if (k + 1 < steps) p.load(lds + ((k + 1) & 1) * S::kStage);
+    p.load(lds + ((k + 1) & 1) * S::kStage, k + 1, k + 1 < steps);
     p.mul(f);
   }
   // this lane's rows m, columns n .. n + 4 TN
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
   const int64_t lto = row_bytes(cols);
   constexpr int P = S::BM + 4;   // LDS row of the transposed tile, words
   unsigned* tr = (unsigned*)lds;
-  __syncthreads();
+  stage_ready();
   const float unscale = STEP == kStepA ? kScaleA / (g.s * g.s) : 1.0f;
   const float lr = STEP == kStepLast ? (bt.lr_dev ? *bt.lr_dev : bt.lr) : 0.0f;
   const bool tall = g.m > g.n;

@@ -13,7 +13,7 @@
 // A lane's two 16-byte pieces of a chunk (piece g and g + 4, g = lane / 16) are
 // then the whole operand of either form, so staging and reading are the same.
 //
-// Staging: global_load_lds (16 B per lane, no VGPRs) into two LDS stages; the
+// Staging: buffer loads into LDS (16 B per lane, no VGPRs) into two LDS stages; the
 // next stage's loads are issued after this stage's fragment reads (the compiler
 // waits for every outstanding LDS load before an LDS read) and land under its
 // MFMAs. Piece p of row r lies at p ^ swz(r), so the 16 rows that a fragment
@@ -61,6 +61,17 @@ __device__ __forceinline__ f32x4 wide_block(const i32x8& n, const i32x8& m, int 
   return acc;
 }
 
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+  const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// A buffer's range: everything, or nothing. (Opaque to the compiler, which would branch over the
+// loads otherwise.)
+__device__ __forceinline__ int range_of(bool live) { return __builtin_amdgcn_readfirstlane(live ? -1 : 0); }
+
 // TM x TN tiles of 16 x 16 per wave, WR x WC waves.
 template <class MODE, int TM_, int TN_, int WR_, int WC_>
 struct TileShape {
@@ -87,70 +98,99 @@ template <class S>
 struct TileProduct {
   static constexpr int TM = S::TM, TN = S::TN;
   f32x4 acc[TM][TN];
-  const char* pa[S::LA];
-  const char* pb[S::LB];
+  const char* a0;          // the tile's first rows
+  const char* b0;
+  unsigned va[S::LA];      // this thread's pieces: byte offsets from them
+  unsigned vb[S::LB];
 
-  // Rows m0 .. of A and n0 .. of B; rows behind the last one read the last one again
-  // (their results are not stored).
+  // Rows m0 .. (below M) of A and n0 .. (below N) of B; rows behind the last one read the last one
+  // again (their results are not stored). lda, ldb: bytes, 2^24 at most.
   __device__ __forceinline__ void init(const char* A, int64_t lda, int64_t m0, int64_t M, const char* B,
                                        int64_t ldb, int64_t n0, int64_t N) {
     const int t = threadIdx.x;
+    a0 = (const char*)uniform((int64_t)(A + m0 * lda));
+    const int am = (int)(M - 1 - m0 < S::BM ? M - 1 - m0 : S::BM);
 #pragma unroll
     for (int i = 0; i < S::LA; ++i) {
       const int idx = i * S::NT + t, r = idx >> 3, p = (idx & 7) ^ swz<TM>(r);
-      const int64_t row = m0 + r < M ? m0 + r : M - 1;
-      pa[i] = A + row * lda + p * 16;
+      va[i] = (unsigned)(r < am ? r : am) * (unsigned)lda + p * 16;
     }
-#pragma unroll
-    for (int i = 0; i < S::LB; ++i) {
-      const int idx = i * S::NT + t, r = idx >> 3, p = (idx & 7) ^ swz<TN>(r);
-      const int64_t row = n0 + r < N ? n0 + r : N - 1;
-      pb[i] = B + row * ldb + p * 16;
-    }
+    set_n(B, ldb, n0, N);
+    clear();
+  }
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = f32x4(0.0f);
   }
 
-  // Starts the loads of the next chunk into a stage.
-  __device__ __forceinline__ void load(char* stage) {
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-    for (int i = 0; i < S::LA; ++i) {
-      __builtin_amdgcn_global_load_lds(
-          (const void*)pa[i], (__attribute__((address_space(3))) void*)(stage + (i * S::NT + w * 64) * 16), 16,
-          0, 0);
-      pa[i] += 128;
-    }
-    char* sb = stage + S::BM * 128;
+  // The N rows n0 .. (below N) of B instead.
+  __device__ __forceinline__ void set_n(const char* B, int64_t ldb, int64_t n0, int64_t N) {
+    const int t = threadIdx.x;
+    b0 = (const char*)uniform((int64_t)(B + n0 * ldb));
+    const int bm = (int)(N - 1 - n0 < S::BN ? N - 1 - n0 : S::BN);
 #pragma unroll
     for (int i = 0; i < S::LB; ++i) {
-      __builtin_amdgcn_global_load_lds(
-          (const void*)pb[i], (__attribute__((address_space(3))) void*)(sb + (i * S::NT + w * 64) * 16), 16, 0,
-          0);
-      pb[i] += 128;
+      const int idx = i * S::NT + t, r = idx >> 3, p = (idx & 7) ^ swz<TN>(r);
+      vb[i] = (unsigned)(r < bm ? r : bm) * (unsigned)ldb + p * 16;
     }
+  }
+
+  // Starts the loads of chunk k of an operand (M's rows, N's rows) into LDS. `live` false: nothing
+  // is read (an empty range: zeros arrive), so that a loop's last step needs no branch around its
+  // loads; wait for them all the same before the LDS is used again or the wave ends.
+  __device__ __forceinline__ void load_m(char* to, int k, bool live) const { pieces<S::LA>(a0, va, to, k, live); }
+  __device__ __forceinline__ void load_n(char* to, int k, bool live) const { pieces<S::LB>(b0, vb, to, k, live); }
+  __device__ __forceinline__ void load(char* stage, int k, bool live) const {
+    load_m(stage, k, live);
+    load_n(stage + S::BM * 128, k, live);
+  }
+  template <int L>
+  static __device__ __forceinline__ void pieces(const char* base, const unsigned (&v)[L], char* to, int k, bool live) {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k * 128), 0, range_of(live), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (__attribute__((address_space(3))) void*)(to + (i * S::NT + w * 64) * 16), 16, (int)v[i], 0, 0, 0);
   }
 
   struct Frags {
     i32x4 m[TM][2], n[TN][2];
   };
-  __device__ __forceinline__ void read(Frags& f, const char* stage) const {
+  __device__ __forceinline__ void read(Frags& f, const char* stage) const { read(f, stage, stage + S::BM * 128); }
+  __device__ __forceinline__ void read(Frags& f, const char* sa, const char* sb) const {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, a = lane & 15;
     const int wr = (w / S::WC) * 16 * TM, wc = (w % S::WC) * 16 * TN;
-    const char* sb = stage + S::BM * 128;
+    // one N and one M tile in turn: the first products need only the first of each
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int r = wc + tile_row<TN>(j, a);
-      f.n[j][0] = *(const i32x4*)(sb + r * 128 + ((g ^ swz<TN>(r)) << 4));
-      f.n[j][1] = *(const i32x4*)(sb + r * 128 + (((g + 4) ^ swz<TN>(r)) << 4));
+    for (int d = 0; d < (TM > TN ? TM : TN); ++d) {
+      if (d < TN) {
+        const int r = wc + tile_row<TN>(d, a);
+        f.n[d][0] = *(const i32x4*)(sb + r * 128 + ((g ^ swz<TN>(r)) << 4));
+        f.n[d][1] = *(const i32x4*)(sb + r * 128 + (((g + 4) ^ swz<TN>(r)) << 4));
+      }
+      if (d < TM) {
+        const int r = wr + tile_row<TM>(d, a);
+        f.m[d][0] = *(const i32x4*)(sa + r * 128 + ((g ^ swz<TM>(r)) << 4));
+        f.m[d][1] = *(const i32x4*)(sa + r * 128 + (((g + 4) ^ swz<TM>(r)) << 4));
+      }
     }
+  }
+
+  // The products in growing squares (i, j <= d), as their operands arrive.
+  template <class F>
+  static __device__ __forceinline__ void squares(F f) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int r = wr + tile_row<TM>(i, a);
-      f.m[i][0] = *(const i32x4*)(stage + r * 128 + ((g ^ swz<TM>(r)) << 4));
-      f.m[i][1] = *(const i32x4*)(stage + r * 128 + (((g + 4) ^ swz<TM>(r)) << 4));
+    for (int d = 0; d < (TM > TN ? TM : TN); ++d) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        if (j < d && d < TM) f(d, j);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        if (i <= d && d < TN) f(i, d);
     }
   }
 
@@ -160,34 +200,25 @@ struct TileProduct {
 
   // Fp8, Fp8Wide: sm[i] / sn: the rows' scales in the lowest byte (E8M0).
   __device__ __forceinline__ void mul(const Frags& f, const int (&sm)[TM], int sn) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const i32x8 m = join(f.m[i]);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if constexpr (std::is_same<typename S::Mode, Fp8Wide>::value)
-          acc[i][j] = wide_block(join(f.n[j]), m, sn & 255, sm[i] & 255, acc[i][j]);
-        else
-          acc[i][j] =
-              __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(f.n[j]), m, acc[i][j], 0, 0, 0, sn, 0, sm[i]);
-      }
-    }
+    squares([&](int i, int j) {
+      if constexpr (std::is_same<typename S::Mode, Fp8Wide>::value)
+        acc[i][j] = wide_block(join(f.n[j]), join(f.m[i]), sn & 255, sm[i] & 255, acc[i][j]);
+      else
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(f.n[j]), join(f.m[i]), acc[i][j], 0, 0, 0,
+                                                                     sn, 0, sm[i]);
+    });
   }
 
   __device__ __forceinline__ void mul(const Frags& f) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    squares([&](int i, int j) {
       const f16x8 mh = __builtin_bit_cast(f16x8, f.m[i][0]), ml = __builtin_bit_cast(f16x8, f.m[i][1]);
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const f16x8 nh = __builtin_bit_cast(f16x8, f.n[j][0]), nl = __builtin_bit_cast(f16x8, f.n[j][1]);
-        f32x4 c = acc[i][j];
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nh, mh, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nl, mh, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nh, ml, c, 0, 0, 0);
-        acc[i][j] = c;
-      }
-    }
+      const f16x8 nh = __builtin_bit_cast(f16x8, f.n[j][0]), nl = __builtin_bit_cast(f16x8, f.n[j][1]);
+      f32x4 c = acc[i][j];
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nh, mh, c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nl, mh, c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nh, ml, c, 0, 0, 0);
+      acc[i][j] = c;
+    });
   }
 
   // This lane's result rows and columns within the workgroup's tile: tile i -> row m(i),
@@ -213,6 +244,16 @@ __device__ __forceinline__ void stage_ready() {
 __device__ __forceinline__ int64_t xcd_tile(int64_t p, int64_t total) {
   const int64_t q = total / 8, rem = total % 8, x = p % 8, i = p / 8;
   return x * q + (x < rem ? x : rem) + i;
+}
+
+// The order in which an XCD walks mtiles x ntiles: bands of `band` row tiles, down a band's
+// column before the next one, so that the tiles in flight form a patch and share both operands in L2.
+__device__ __forceinline__ void band_tile(int64_t id, int mtiles, int ntiles, int band, int& mt, int& nt) {
+  const int64_t per = (int64_t)band * ntiles;
+  const int b = (int)(id / per), m0 = b * band, h = mtiles - m0 < band ? mtiles - m0 : band;
+  const int r = (int)(id - b * per);
+  nt = r / h;
+  mt = m0 + r - nt * h;
 }
 
 }  // namespace nerfhip

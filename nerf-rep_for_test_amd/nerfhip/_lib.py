@@ -102,7 +102,7 @@ SIGNATURES = {
                                           _S]),
     "nerf_muon_workspace": (_SZ, [_P, _I]),
     "nerf_muon": (_I, [_P, _I, _P, _P, _SZ, _S]),
-    "nerf_fp8_linear_workspace": (_SZ, [_I64, _I64, _I, _I]),
+    "nerf_fp8_linear_workspace": (_SZ, [_I64, _I64, _I64, _I, _I]),
     "nerf_fp8_linear": (_I, [_P, _P, _SZ, _S]),
     "nerf_fp8_quantize_weight": (_I, [_P, _I, _I64, _I64, _I, _I64, _I64, _P, _P, _S]),
 }

@@ -118,7 +118,7 @@ def launch(x, weight, M, order, slots, offsets, bias, relu, out_dtype, who):
     E = weight.q.shape[0] if weight.q.dim() == 3 else 1
     d = _Fp8Linear(ptr(x), x.stride(0), x.shape[0], ptr(order), TYPES[x.dtype], TYPES[out_dtype], slots, E,
                    int(relu), M, N, K, ptr(weight.q), ptr(weight.scale), ptr(offsets), ptr(bias), ptr(out), N)
-    need = _lib.lib().nerf_fp8_linear_workspace(M, K, E, int(offsets is not None))
+    need = _lib.lib().nerf_fp8_linear_workspace(M, N, K, E, int(offsets is not None))
     with on_device_of(x):
         ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
         call("nerf_fp8_linear", ctypes.addressof(d), ptr(ws), need, _lib.stream_of(x.device))

@@ -88,6 +88,9 @@ def test_quantize_weight(dev, E, N, K, dt):
 
 SHAPES = [(1, 1, 1), (1, 64, 128), (3, 17, 130), (16, 40, 1000), (17, 33, 64), (16, 4096, 4096), (129, 200, 257),
           (777, 1000, 1111), (300, 128, 2048), (1, 1000, 8192), (4097, 256, 256), (130, 130, 20000)]
+LARGE = [(65537, 100, 260, torch.bfloat16), (65536, 256, 256, torch.float16), (65600, 300, 130, torch.float32),
+         (70000, 40, 500, torch.bfloat16), (4100, 8200, 4224, torch.bfloat16), (3, 5, 66000, torch.float32),
+         (140, 150, 66000, torch.bfloat16)]
 
 
 @pytest.mark.parametrize("M,N,K,dt", [(*s, dt) for s in SHAPES for dt in (torch.bfloat16, torch.float32, torch.float16)
@@ -106,6 +109,21 @@ def test_linear(dev, M, N, K, dt):
     wide = torch.zeros(M, K + 3, dtype=dt)
     wide[:, 1:K + 1] = x
     assert torch.equal(fp8.linear(wide.to(dev)[:, 1:K + 1], f), fp8.linear(x.to(dev), f))
+
+
+@pytest.mark.parametrize("M,N,K,dt", LARGE)
+def test_linear_large(dev, M, N, K, dt):
+    """The forms for many short rows, long rows with many tiles, and more blocks than scales fit into LDS:
+    rows from all over, against 64 bits."""
+    from nerfhip import fp8
+    g = torch.Generator(device="cuda").manual_seed(M)
+    f = fp8.quantize_weight(torch.randn(N, K, device=dev, generator=g) * K ** -0.5)
+    x = torch.randn(M, K, device=dev, generator=g).to(dt)
+    bias = torch.randn(N, device=dev, generator=g)
+    y = fp8.linear(x, f, bias=bias)
+    rows = torch.unique(torch.cat([torch.arange(0, M, max(1, M // 150)), torch.arange(max(0, M - 130), M)]))
+    check(y[rows.to(dev)], rows8(x[rows.to(dev)].cpu()), f.dequantize().cpu().double(), bias.cpu(), False, dt)
+    assert bool(torch.isfinite(y).all())
 
 
 def test_linear_takes_any_leading_axes_and_layouts(dev):
@@ -154,7 +172,8 @@ def test_extreme_and_non_finite_values(dev, M):
 
 
 @pytest.mark.parametrize("T,k,E,N,K", [(1, 1, 1, 16, 16), (1, 4, 8, 100, 200), (16, 6, 64, 96, 256), (40, 2, 3, 130, 129),
-                                       (600, 3, 5, 200, 384), (64, 1, 300, 16, 128), (257, 2, 2, 128, 1000)])
+                                       (600, 3, 5, 200, 384), (64, 1, 300, 16, 128), (257, 2, 2, 128, 1000),
+                                       (16500, 4, 7, 130, 200)])
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_expert_linear(dev, T, k, E, N, K, dt):
     from nerfhip import experts
