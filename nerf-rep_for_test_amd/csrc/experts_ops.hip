@@ -1,6 +1,8 @@
 // Gated experts: the gate that routes each row to k of E experts, the plan that
 // sorts the (row, choice) slots by expert, and the join of the experts' outputs;
 // with the backward passes of gate and join.
+#include <type_traits>
+
 #include "common.h"
 
 namespace nerfhip {
@@ -33,6 +35,10 @@ struct alignas(sizeof(T) * N) Vec {
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) {
   return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+  return __uint_as_float(dpp<CTRL>(__float_as_uint(v)));
 }
 template <int L, class OP>
 __device__ __forceinline__ unsigned reduce32(unsigned v, OP op) {
@@ -68,28 +74,60 @@ __device__ __forceinline__ double row_sum(double v) {
   return v;
 }
 
-// (key, index) with the higher key, or at equal keys the lower index, over the lanes of a row.
-template <int L>
-__device__ __forceinline__ void row_best(float& key, int& idx) {
-  // ordered as unsigned: sign bit flipped, negatives inverted; the index inverted below it
-  const unsigned b = __float_as_uint(key + 0.0f);   // (-0 counts as 0)
-  unsigned hi = b ^ ((unsigned)((int)b >> 31) | 0x80000000u), lo = ~(unsigned)idx;
-  auto step = [&](unsigned h, unsigned l) {
-    const bool other = h > hi || (h == hi && l > lo);
-    hi = other ? h : hi;
-    lo = other ? l : lo;
-  };
-  step(dpp<0xB1>(hi), dpp<0xB1>(lo));
-  step(dpp<0x4E>(hi), dpp<0x4E>(lo));
-  step(dpp<0x141>(hi), dpp<0x141>(lo));
-  step(dpp<0x140>(hi), dpp<0x140>(lo));
-  if constexpr (L == 64) {
-    step((unsigned)__shfl_xor((int)hi, 16), (unsigned)__shfl_xor((int)lo, 16));
-    step((unsigned)__shfl_xor((int)hi, 32), (unsigned)__shfl_xor((int)lo, 32));
-  }
-  key = __uint_as_float(hi & 0x80000000u ? hi ^ 0x80000000u : ~hi);
-  idx = (int)~lo;
+// LDS written by a row's lanes (all of one wave) may be read by them.
+__device__ __forceinline__ void row_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
 }
+
+// A key and its expert as one positive number: 2^52 + (the key's bits in rising order, 32 bits) * 1024 +
+// (1023 - expert). Larger: the higher key, or at equal keys the lower index. One v_max_f64 compares
+// both (its rate is FP32's), and a comparison of sorting is two instructions.
+__device__ __forceinline__ double pack_key(float key, int e) {
+  const unsigned b = __float_as_uint(key + 0.0f);   // (-0 counts as 0)
+  const unsigned u = b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+  return __hiloint2double((int)(0x43300000u | u >> 22), (int)(u << 10 | (unsigned)(1023 - e)));
+}
+__device__ __forceinline__ int index_of(double p) { return 1023 - (__double2loint(p) & 1023); }
+__device__ __forceinline__ float key_of(double p) {
+  const unsigned u = (unsigned)__double2hiint(p) << 22 | (unsigned)__double2loint(p) >> 10;
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  return __hiloint2double((int)dpp<CTRL>((unsigned)__double2hiint(v)), (int)dpp<CTRL>((unsigned)__double2loint(v)));
+}
+template <int L>
+__device__ __forceinline__ double row_max(double v) {
+  v = fmax(v, dpp64<0xB1>(v));
+  v = fmax(v, dpp64<0x4E>(v));
+  v = fmax(v, dpp64<0x141>(v));
+  v = fmax(v, dpp64<0x140>(v));
+  if constexpr (L == 64) {
+    v = fmax(v, __shfl_xor(v, 16));
+    v = fmax(v, __shfl_xor(v, 32));
+  }
+  return v;
+}
+// A sorting network (merge exchange) for a power of two of values, the largest first.
+template <int N>
+__device__ __forceinline__ void sort_down(double (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const double hi = fmax(v[i + j], v[i + j + k]), lo = fmin(v[i + j], v[i + j + k]);
+            v[i + j] = hi;
+            v[i + j + k] = lo;
+          }
+}
+
+// (key, index) with the higher key, or at equal keys the lower index, over the lanes of a row.
 template <int L>
 __device__ __forceinline__ void row_best(double& key, int& idx) {
   for (int d = 1; d < L; d *= 2) {
@@ -117,125 +155,221 @@ __device__ __forceinline__ int expert_of(int lane, int v) {
   return ((v >> 2) * L + lane) * 4 + (v & 3);
 }
 
-// Chooses a row's k experts (into chosen[], the same in all of its lanes' view of LDS). In 32 bits
-// (F = float) it returns whether the order could be another one in exact arithmetic: two
-// neighbours in the order (or the last kept and first dropped group) nearer than the keys' error
-// and not made of equal inputs. Such rows are done again with F = double, so the choice is that
-// of exact arithmetic while nearly every row pays for 32 bits only. Without a bias the keys are
-// the logits themselves and nothing but groups' sums can be in doubt.
-template <class F, int L, int V, class T>
-__device__ bool choose(const RouteArgs& a, const T* row, const float (&x)[V], float top, float* keys, int* chosen,
-                       int lane) {
-  constexpr bool k32 = sizeof(F) == 4;
-  F key[V];
-  const bool scored = a.bias != nullptr || (a.groups > 1 && a.group_top2);
-  F sum = 0;
-  if (scored) {
-    if (a.sigmoid) {
+// The scores s of a lane's logits, in F.
+template <class F, int L, int V>
+__device__ __forceinline__ void scores(const RouteArgs& a, const float (&x)[V], float top, int lane, F (&s)[V]) {
+  if (a.sigmoid) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) key[v] = (F)1 / ((F)1 + exp_of(-(F)x[v]));
-    } else {
+    for (int v = 0; v < V; ++v) s[v] = (F)1 / ((F)1 + exp_of(-(F)x[v]));
+  } else {
+    F sum = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        key[v] = expert_of<L>(lane, v) < a.E ? exp_of((F)x[v] - (F)top) : (F)0;
-        sum += key[v];
-      }
-      sum = row_sum<L>(sum);
-#pragma unroll
-      for (int v = 0; v < V; ++v) key[v] = key[v] / sum;
+    for (int v = 0; v < V; ++v) {
+      s[v] = expert_of<L>(lane, v) < a.E ? exp_of((F)x[v] - (F)top) : (F)0;
+      sum += s[v];
     }
-    if (a.bias) {
+    sum = (F)1 / row_sum<L>(sum);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int e = expert_of<L>(lane, v);
-        if (e < a.E) key[v] += (F)a.bias[e];
-      }
+    for (int v = 0; v < V; ++v) s[v] *= sum;
+  }
+}
+
+// NaN and -inf as the lowest number: in order before what is out of reach (-inf).
+template <class F>
+__device__ __forceinline__ F ranked(F key) {
+  return key > lowest<F>() ? key : lowest<F>();
+}
+
+// The groups that stay (bits) by the highest or two highest of their keys; `doubt`: whether the last
+// one kept and the first one dropped are nearer than `tol`.
+template <class F, int L, int V>
+__device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, const F (&key)[V], F* ks, int lane, F tol,
+                                                          bool& doubt) {
+  const int per = a.E / a.groups;
+  F* gs = ks + a.E + a.groups;
+  auto score = [&](F b1, F b2) { return a.group_top2 && per > 1 ? (b2 > lowest<F>() ? b1 + b2 : lowest<F>()) : b1; };
+  if (sizeof(F) == 4 && per >= 4 && per <= 64 && (per & (per - 1)) == 0) {
+    // a group is whole lanes' runs of 4: the two highest by DPP
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      float b1 = -__builtin_inff(), b2 = b1;
+      auto add = [&](float o1, float o2) {
+        b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+        b1 = fmaxf(b1, o1);
+      };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) add((float)key[v + i], -__builtin_inff());
+      if (per > 4) add(dpp_f<0xB1>(b1), dpp_f<0xB1>(b2));
+      if (per > 8) add(dpp_f<0x4E>(b1), dpp_f<0x4E>(b2));
+      if (per > 16) add(dpp_f<0x141>(b1), dpp_f<0x141>(b2));
+      if (per > 32) add(dpp_f<0x140>(b1), dpp_f<0x140>(b2));
+      const int e = expert_of<L>(lane, v);
+      if (e < a.E && e % per == 0) gs[e / per] = score(b1, b2);
     }
   } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = (F)x[v];
-  }
-  // NaN and -inf as the lowest number: in order before what is out of reach (-inf)
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    key[v] = key[v] > lowest<F>() ? key[v] : lowest<F>();
-    if (expert_of<L>(lane, v) >= a.E) key[v] = -(F)__builtin_inff();
-  }
-  bool doubt = false;
-  // twice what two keys (or groups' sums of two keys) can be off in 32 bits: the scores (at most 1) by
-  // 1e-6 with the error of the softmax's sum, each addition by half a step
-  auto near = [&](F p, F q) { return p - q < (F)4e-6 + (F)4.8e-7 * (p < 0 ? -p : p); };
-  if (a.groups > 1) {
-    // the row's keys through LDS: lane j < groups takes group j
-    F* ks = (F*)keys;
+    // through LDS, lane j takes group j
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int e = expert_of<L>(lane, v);
-      if (e < a.E) ks[e] = key[v];
+      if (e < a.E) ks[e + e / per] = key[v];   // (a word between groups: they lie in different banks)
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    const int per = a.E / a.groups;
-    F* gs = ks + a.E;
+    row_fence();
     for (int j = lane; j < a.groups; j += L) {
       F b1 = -(F)__builtin_inff(), b2 = b1;
+#pragma unroll 8
       for (int i = 0; i < per; ++i) {
-        const F v = ks[j * per + i];
+        const F v = ks[j * (per + 1) + i];
         b2 = v > b1 ? b1 : (v > b2 ? v : b2);
         b1 = v > b1 ? v : b1;
       }
-      gs[j] = a.group_top2 && per > 1 ? (b1 > lowest<F>() / 2 && b2 > lowest<F>() / 2 ? b1 + b2 : lowest<F>()) : b1;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    unsigned long long keep = 0;
-    F last = __builtin_inff(), first = -(F)__builtin_inff();   // lowest kept, highest dropped
-    for (int j = 0; j < a.groups; ++j) {
-      const F mine = gs[j];
-      int better = 0;
-      for (int i = 0; i < a.groups; ++i) better += gs[i] > mine || (gs[i] == mine && i < j);
-      if (better < a.top_groups) {
-        keep |= 1ull << j;
-        last = mine < last ? mine : last;
-      } else {
-        first = mine > first ? mine : first;
-      }
-    }
-    // (max of logits without a bias: exact)
-    if (k32 && scored && a.top_groups < a.groups && first > lowest<F>() / 2) doubt = near(last, first);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = expert_of<L>(lane, v);
-      if (!a.bias && e < a.E) key[v] = (F)x[v] > lowest<F>() ? (F)x[v] : lowest<F>();   // the order of the logits
-      if (e < a.E && !((keep >> (e / per)) & 1)) key[v] = -(F)__builtin_inff();
+      gs[j] = score(b1, b2);
     }
   }
-  const int rounds = k32 && a.bias && a.k < a.E ? a.k + 1 : a.k;   // one more: the first one left out
-  F before = __builtin_inff();
-  int ib = -1;
-  for (int j = 0; j < rounds; ++j) {
-    F best = -(F)__builtin_inff();
-    int idx = 0x7fffffff;
+  row_fence();
+  // a lane ranks its own groups; all of the row's lanes join their bits
+  unsigned lo = 0, hi = 0;
+  F last = __builtin_inff(), first = -(F)__builtin_inff();   // lowest kept, highest dropped
+  for (int j = lane; j < a.groups; j += L) {
+    const F mine = gs[j];
+    int better = 0;
+    for (int i = 0; i < a.groups; ++i) better += gs[i] > mine || (gs[i] == mine && i < j);
+    if (better < a.top_groups) {
+      lo |= j < 32 ? 1u << j : 0u;
+      hi |= j < 32 ? 0u : 1u << (j - 32);
+      last = mine < last ? mine : last;
+    } else {
+      first = mine > first ? mine : first;
+    }
+  }
+  const unsigned long long keep = (unsigned long long)row_or<L>(hi) << 32 | row_or<L>(lo);
+  if (sizeof(F) == 4) {
+    last = -row_max<L>((float)-last);
+    first = row_max<L>((float)first);
+    doubt = a.top_groups < a.groups && first > lowest<F>() && last - first < tol + (F)4.8e-7 * (last < 0 ? -last : last);
+  }
+  return keep;
+}
+
+// Chooses a row's k experts (into chosen[] in LDS, which its lanes read after a row_fence).
+//
+// The order is that of exact arithmetic. Without a bias the keys are the logits themselves; with
+// one they are computed in 32 bits, and where two neighbours in the order (or the last group kept
+// and the first one dropped) are nearer than the keys' error and not made of equal inputs, in
+// 64 bits again: then only for the experts that can be among the first k (scores of a softmax: for
+// all, its sum takes them all). Nearly every row pays for 32 bits only.
+template <int L, int V, class T>
+__device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const float (&x)[V], float top, double* lds, int* chosen,
+                       int lane) {
+  float key[V];
+  float tol = 0.0f;   // twice two keys' errors, apart from their last rounding
+  const bool scored = a.bias != nullptr || (a.groups > 1 && a.group_top2);
+  const int per = a.E / a.groups;
+  if (scored) {
+    scores<float, L, V>(a, x, top, lane, key);
+    // sigmoid: 3 steps of a score (at most 1). Softmax: 1.2e-6 of one (the sum of 1024 terms: 20 steps),
+    // the row's largest at most
+    float most = 0.0f;
+    if (!a.sigmoid) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) most = fmaxf(most, key[v]);
+      most = row_max<L>(most);
+    }
+    tol = a.sigmoid ? 8e-7f : 5e-6f * most;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int e = expert_of<L>(lane, v);
-      const bool b = key[v] > best || (key[v] == best && e < idx);
-      best = b ? key[v] : best;
-      idx = b ? e : idx;
+      key[v] = e < a.E ? ranked(a.bias ? key[v] + a.bias[e] : key[v]) : -__builtin_inff();
     }
-    row_best<L>(best, idx);
-    if (k32 && a.bias && j > 0 && best > lowest<F>() && near(before, best))
-      doubt = doubt || !((float)row[ib] == (float)row[idx] && a.bias[ib] == a.bias[idx]);
-    before = best;
-    ib = idx;
-    if (j < a.k && lane == 0) chosen[j] = idx;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = expert_of<L>(lane, v) < a.E ? ranked(x[v]) : -__builtin_inff();
+  }
+  unsigned long long keep = ~0ull;
+  if (a.groups > 1) {
+    bool doubt = false;
+    // (the highest logits without a bias: exact)
+    keep = keep_groups<float, L, V>(a, key, (float*)lds, lane, 2.0f * tol, doubt);
+    if (doubt && scored) {
+      double k64[V];
+      scores<double, L, V>(a, x, top, lane, k64);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int e = expert_of<L>(lane, v);
+        k64[v] = e < a.E ? ranked(a.bias ? k64[v] + (double)a.bias[e] : k64[v]) : -(double)__builtin_inff();
+      }
+      row_fence();
+      keep = keep_groups<double, L, V>(a, k64, lds, lane, 0.0, doubt);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = expert_of<L>(lane, v);
+      if (e < a.E) {
+        if (!a.bias) key[v] = ranked(x[v]);   // the order of the logits
+        if (!((keep >> (e / per)) & 1)) key[v] = -__builtin_inff();
+      }
+    }
+  }
+  bool doubt = false;
+  float before = __builtin_inff();
+  int ib = 0;
+  const int rounds = a.bias && a.k < a.E ? a.k + 1 : a.k;   // one more: the first one left out
+  double order[V];   // a lane's keys, highest first
+#pragma unroll
+  for (int v = 0; v < V; ++v) order[v] = pack_key(key[v], expert_of<L>(lane, v));
+  sort_down<V>(order);
+  auto take = [&](auto depth) {   // (a lane gives at most `rounds` of its keys)
+    constexpr int D = decltype(depth)::value;
+    for (int j = 0; j < rounds; ++j) {
+      const double first = row_max<L>(order[0]);
+      const bool mine = order[0] == first;
+#pragma unroll
+      for (int v = 0; v + 1 < D; ++v) order[v] = mine ? order[v + 1] : order[v];
+      order[D - 1] = mine ? 0.0 : order[D - 1];
+      const float best = key_of(first);
+      const int idx = index_of(first);
+      if (a.bias && j > 0 && best > lowest<float>() && before - best < tol + 2.4e-7f * fabsf(before))
+        doubt = doubt || !((float)row[ib] == (float)row[idx] && a.bias[ib] == a.bias[idx]);
+      if (j < a.k) {
+        before = best;
+        ib = idx;
+        if (lane == 0) chosen[j] = idx;
+      }
+    }
+  };
+  if (V > 9 && rounds <= 9) take(std::integral_constant<int, (V > 9 ? 9 : V)>());
+  else take(std::integral_constant<int, V>());
+  if (!doubt) return;
+  // 64 bits, for the experts that may be among the first k: not below the k-th by more than the error
+  const float least = fmaxf(before - tol - 2.4e-7f * fabsf(before), lowest<float>());
+  double k64[V];
+  if (a.sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      k64[v] = -(double)__builtin_inff();
+      if (key[v] >= least) k64[v] = ranked(1.0 / (1.0 + exp(-(double)x[v])) + (double)a.bias[expert_of<L>(lane, v)]);
+    }
+  } else {
+    scores<double, L, V>(a, x, top, lane, k64);
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (expert_of<L>(lane, v) == idx) {
-        key[v] = -(F)__builtin_inff();
-      }
+      k64[v] = key[v] >= least ? ranked(k64[v] + (double)a.bias[expert_of<L>(lane, v)]) : -(double)__builtin_inff();
   }
-  return doubt;
+  row_fence();
+  for (int j = 0; j < a.k; ++j) {
+    double best = -(double)__builtin_inff();
+    int idx = 0x7fffffff;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (k64[v] > best) {
+        best = k64[v];
+        idx = expert_of<L>(lane, v);
+      }
+    row_best<L>(best, idx);
+    if (lane == 0) chosen[j] = idx;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (expert_of<L>(lane, v) == idx) k64[v] = -(double)__builtin_inff();
+  }
 }
 
 // A chosen expert's part in the weights, r_j of the formulas: w_j = scale * r_j.
@@ -276,8 +410,8 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   constexpr int R = 256 / L;
   const int lane = threadIdx.x % L, r = threadIdx.x / L;
   const int64_t t = (int64_t)blockIdx.x * R + r;
-  const int per_row = a.groups > 1 ? a.E + a.groups : 0;
-  float* keys = (float*)(route_lds + (int64_t)r * per_row);
+  const int per_row = a.groups > 1 ? a.E + 2 * a.groups : 0;
+  double* keys = route_lds + (int64_t)r * per_row;
   int* chosen = (int*)(route_lds + (int64_t)R * per_row) + r * kMaxChoices;
   // (a workgroup's last rows may lie behind T: they do the last row again and store nothing, so that
   // a wave's lanes stay together)
@@ -294,36 +428,43 @@ __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   }
   top = row_max<L>(top);
   bad = row_or<L>(bad) | (!a.sigmoid && top == __builtin_inff());
-  if (choose<float, L, V>(a, row, x, top, keys, chosen, lane)) choose<double, L, V>(a, row, x, top, keys, chosen, lane);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-  __builtin_amdgcn_wave_barrier();
-  float m = -__builtin_inff();
+  choose<L, V>(a, row, x, top, keys, chosen, lane);
+  row_fence();
+  // lane j holds choice j (and j + L)
+  constexpr int C = kMaxChoices / L > 1 ? kMaxChoices / L : 1;
+  int e[C];
+  float l[C], m = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int j = lane + c * L;
+    e[c] = j < a.k ? chosen[j] : 0;
+    l[c] = j < a.k ? (float)row[e[c]] : -__builtin_inff();
+    m = fmaxf(m, l[c]);
+  }
   if (a.renorm) {
-    for (int j = lane; j < a.k; j += L) m = fmaxf(m, (float)row[chosen[j]]);
     m = row_max<L>(m);
     if (a.sigmoid) m = fminf(m, 0.0f);
-  } else {
-    m = top;
-  }
-  float sum = 0.0f;
-  if (a.renorm) {
-    for (int j = lane; j < a.k; j += L) sum += chosen_part(a, (float)row[chosen[j]], m);
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum += lane + c * L < a.k ? chosen_part(a, l[c], m) : 0.0f;
     sum = row_sum<L>(sum);
   } else if (!a.sigmoid) {
+    m = top;
 #pragma unroll
     for (int v = 0; v < V; ++v) sum += expert_of<L>(lane, v) < a.E ? expf(x[v] - top) : 0.0f;
     sum = row_sum<L>(sum);
   } else {
+    m = top;
     sum = 1.0f;
   }
   const bool nothing = m == -__builtin_inff();   // every (chosen) logit is -inf
-  if (t < a.T) {
-    for (int j = lane; j < a.k; j += L) {
-      const int e = chosen[j];
-      float w = nothing ? 0.0f : chosen_part(a, (float)row[e], m) / sum * a.scale;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int j = lane + c * L;
+    if (t < a.T && j < a.k) {
+      float w = nothing ? 0.0f : chosen_part(a, l[c], m) / sum * a.scale;
       if (bad) w = __builtin_nanf("");
       a.weights[t * a.k + j] = w;
-      a.experts[t * a.k + j] = e;
+      a.experts[t * a.k + j] = e[c];
     }
   }
 }
@@ -391,8 +532,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const RouteBwdArgs 
     }
     dot = row_sum<L>(dot);
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-  __builtin_amdgcn_wave_barrier();
+  row_fence();
   for (int j = lane; j < a.k; j += L) {
     const int e = ex[j];
     if (e >= 0 && e < a.E) {
@@ -407,8 +547,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const RouteBwdArgs 
       buf[e] = d * a.scale;
     }
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-  __builtin_amdgcn_wave_barrier();
+  row_fence();
   if (t < a.T) {
     T* out = (T*)b.dlogits + t * a.E;
 #pragma unroll
@@ -449,7 +588,7 @@ __device__ __forceinline__ unsigned long long same_expert(int e, bool live, int 
   return peers;
 }
 
-constexpr int kPlanSegs = 256;    // runs of slots (one wave each) of a large plan
+constexpr int kPlanSegs = 1024;   // runs of slots (one wave each) of a large plan
 constexpr int kPlanSmall = 4096;  // up to here one workgroup does everything (LDS: 18 words an expert)
 bool plan_is_small(int64_t n, int E) { return n <= kPlanSmall && E <= 512; }
 
@@ -558,24 +697,32 @@ __global__ __launch_bounds__(64) void plan_count_kernel(const int* experts, int6
 
 // One wave for each expert: its runs' counts become where they begin; totals [E].
 __global__ __launch_bounds__(64) void plan_scan_kernel(int* counts, int* totals) {
-  int4* row = (int4*)(counts + (int64_t)blockIdx.x * kPlanSegs);
-  const int lane = threadIdx.x;
-  static_assert(kPlanSegs == 256, "4 counts for each of 64 lanes");
-  int4 c = row[lane];
-  const int mine = c.x + c.y + c.z + c.w;
+  constexpr int Q = kPlanSegs / 256;
+  int4* row = (int4*)(counts + (int64_t)blockIdx.x * kPlanSegs) + threadIdx.x * Q;
+  int4 c[Q];
+  int mine = 0;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    c[q] = row[q];
+    mine += c[q].x + c[q].y + c[q].z + c[q].w;
+  }
   int sum = mine;
   for (int d = 1; d < 64; d *= 2) {
     const int o = __shfl_up(sum, d);
-    if (lane >= d) sum += o;
+    if ((int)threadIdx.x >= d) sum += o;
   }
-  if (lane == 63) totals[blockIdx.x] = sum;
+  if (threadIdx.x == 63) totals[blockIdx.x] = sum;
   sum -= mine;
-  int4 o;
-  o.x = sum;
-  o.y = o.x + c.x;
-  o.z = o.y + c.y;
-  o.w = o.z + c.z;
-  row[lane] = o;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    int4 o;
+    o.x = sum;
+    o.y = o.x + c[q].x;
+    o.z = o.y + c[q].y;
+    o.w = o.z + c[q].z;
+    sum = o.w + c[q].w;
+    row[q] = o;
+  }
 }
 
 __global__ __launch_bounds__(256) void plan_place_kernel(const int* experts, int64_t n, int64_t seg, int E, int bits,
@@ -738,14 +885,18 @@ void go_route(const RouteArgs& a, const float* dw, void* dlogits, hipStream_t st
     RouteBwdArgs b{a, dw, dlogits};
     hipLaunchKernelGGL((route_backward_kernel<L, V, T, VEC>), grid, dim3(256), R * V * L * 4, st, b);
   } else {
-    const size_t lds = (size_t)R * (a.groups > 1 ? a.E + a.groups : 0) * 8 + R * kMaxChoices * 4;
+    const size_t lds = (size_t)R * (a.groups > 1 ? a.E + 2 * a.groups : 0) * 8 + R * kMaxChoices * 4;
     hipLaunchKernelGGL((route_kernel<L, V, T, VEC>), grid, dim3(256), lds, st, a);
   }
 }
 
 template <class T, bool VEC>
 void go_route_e(const RouteArgs& a, const float* dw, void* dl, hipStream_t st) {
-  if (a.E <= 64) go_route<16, 4, T, VEC>(a, dw, dl, st);
+  // 16 lanes for a row waste least (E = 256, k = 8, T = 65536: 32 us against 59 with 64 lanes), but with
+  // many experts and few rows the time is one row's, which more lanes shorten (T = 1021, sigmoid, bias and
+  // groups: 12.8 us against 18.9; at T = 4096 15.8 against 19.1, at 16384 34 against 30)
+  if (a.E > 128 && a.E <= 256 && a.T <= 4096) go_route<64, 4, T, VEC>(a, dw, dl, st);
+  else if (a.E <= 64) go_route<16, 4, T, VEC>(a, dw, dl, st);
   else if (a.E <= 128) go_route<16, 8, T, VEC>(a, dw, dl, st);
   else if (a.E <= 256) go_route<16, 16, T, VEC>(a, dw, dl, st);
   else if (a.E <= 512) go_route<64, 8, T, VEC>(a, dw, dl, st);

@@ -44,6 +44,14 @@ __device__ __forceinline__ unsigned max16(unsigned v) {
   return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
 }
 
+// The largest value of the 4 lanes that are 16 apart.
+__device__ __forceinline__ unsigned max4(unsigned v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+
 template <class T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
@@ -457,81 +465,99 @@ __global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int
 // ---------------------------------------------------------------- skinny form
 
 // Few rows for each weight matrix: bound by the weights' bytes. A workgroup of 8 waves
-// takes 16 weight rows; the waves share the blocks of K between them, read the weights
-// straight into the matrix operands (16 rows x 128 B lines, no LDS) and quantise the
-// activations in registers (a row's block lies in 4 lanes), so one launch reads each
-// weight once. The 8 partial sums are added in wave order.
-template <class T, class O, int RT, bool VEC>
+// takes 16 TN weight rows; the waves share the blocks of K between them, U at a time (all
+// of their loads in flight), read the weights straight into the matrix operands (16 rows x
+// 128 B lines, no LDS) and quantise the activations in registers (a row's block lies in 4
+// lanes), so one launch reads each weight once. The 8 partial sums are added in wave order.
+template <class T, class O, int TN, bool VEC>
 __global__ __launch_bounds__(512) void skinny_kernel(const LinearArgs a) {
-  constexpr int W = 8;
-  __shared__ float part[W][RT][16][17];
+  constexpr int W = 8, U = TN == 4 ? 1 : 2;
+  __shared__ float part[W][TN][16][17];
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, g = lane >> 4, r = lane & 15;
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * TN;
   const int e = blockIdx.y;
   int64_t lo, hi;
   expert_rows(a, e, lo, hi);
   if (lo >= hi) return;
   const bool none = a.offsets && e == a.E;
-  const int64_t nrow = n0 + r < a.N ? n0 + r : a.N - 1;
   const int eb = none ? 0 : e;
-  const unsigned char* wrow = a.wq + ((int64_t)eb * a.N + nrow) * a.KB * 128 + g * 16;
-  const unsigned char* ws = a.ws + ((int64_t)eb * a.NB + n0 / 128) * a.KB;
-  for (int64_t m0 = lo; m0 < hi; m0 += 16 * RT) {
-    f32x4 acc[RT];
-    const T* xrow[RT];
+  const unsigned char* wrow[TN];
+  const unsigned char* ws = a.ws + ((int64_t)eb * a.NB + n0 / 128) * a.KB;   // (16 TN divides 128)
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      acc[i] = f32x4(0.0f);
-      const int64_t m = m0 + 16 * i + r;
-      const int64_t src = source_row(a.order, a.div, a.x_rows, m < hi ? m : hi - 1);
-      xrow[i] = src < 0 ? nullptr : (const T*)a.x + src * a.ldx;
-    }
-    if (!none) {
-#pragma unroll 4
-      for (int k = w; k < a.KB; k += W) {
-        const i32x4 w0 = *(const i32x4*)(wrow + (int64_t)k * 128);
-        const i32x4 w1 = *(const i32x4*)(wrow + (int64_t)k * 128 + 64);
-        const int sn = ws[k];
-        const i32x8 wf = __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7);
+  for (int j = 0; j < TN; ++j) {
+    const int64_t n = n0 + 16 * j + r;
+    wrow[j] = a.wq + ((int64_t)eb * a.N + (n < a.N ? n : a.N - 1)) * a.KB * 128 + g * 16;
+  }
+  for (int64_t m0 = lo; m0 < hi; m0 += 16) {
+    f32x4 acc[TN];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          float f0[16] = {}, f1[16] = {};
-          if (xrow[i]) {
-            load_row<T, 16, VEC>(f0, xrow[i], (int64_t)k * 128 + g * 16, a.K);
-            load_row<T, 16, VEC>(f1, xrow[i], (int64_t)k * 128 + 64 + g * 16, a.K);
+    for (int j = 0; j < TN; ++j) acc[j] = f32x4(0.0f);
+    const int64_t src = source_row(a.order, a.div, a.x_rows, m0 + r < hi ? m0 + r : hi - 1);
+    const T* xrow = src < 0 ? nullptr : (const T*)a.x + src * a.ldx;
+    for (int k0 = w; k0 < a.KB && !none; k0 += W * U) {
+      i32x4 wf[U][TN][2];
+      int sn[U];
+      T x[U][2][16];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {   // (blocks behind the last one: the last one again, not used)
+        const int64_t k = k0 + u * W < a.KB ? k0 + u * W : a.KB - 1;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          wf[u][j][0] = *(const i32x4*)(wrow[j] + k * 128);
+          wf[u][j][1] = *(const i32x4*)(wrow[j] + k * 128 + 64);
+        }
+        sn[u] = ws[k];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < 16; c += 8) {
+            T v[8] = {};
+            if (xrow) load_raw<T, VEC>(v, xrow, k * 128 + h * 64 + g * 16 + c, a.K);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[u][h][c + q] = v[q];
           }
-          unsigned top = 0;
+      }
 #pragma unroll
-          for (int c = 0; c < 16; ++c) top = max(top, max(abs_bits(f0[c]), abs_bits(f1[c])));
-          top = max(top, (unsigned)__shfl_xor((int)top, 16));
-          top = max(top, (unsigned)__shfl_xor((int)top, 32));
-          const int sc = block_scale(top), ex = 127 - sc;
-          i32x8 xf;
+      for (int u = 0; u < U; ++u) {
+        float f[2][16];
+        unsigned top = 0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            xf[c] = pack4(__builtin_ldexpf(f0[4 * c], ex), __builtin_ldexpf(f0[4 * c + 1], ex),
-                          __builtin_ldexpf(f0[4 * c + 2], ex), __builtin_ldexpf(f0[4 * c + 3], ex));
-            xf[4 + c] = pack4(__builtin_ldexpf(f1[4 * c], ex), __builtin_ldexpf(f1[4 * c + 1], ex),
-                              __builtin_ldexpf(f1[4 * c + 2], ex), __builtin_ldexpf(f1[4 * c + 3], ex));
+        for (int c = 0; c < 32; ++c) {
+          f[c >> 4][c & 15] = (float)x[u][c >> 4][c & 15];
+          top = max(top, abs_bits(f[c >> 4][c & 15]));
+        }
+        top = max4(top);
+        const int sc = block_scale(top), ex = 127 - sc;
+        i32x8 xf;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float* v = &f[c >> 2][(c & 3) * 4];
+          xf[c] = pack4(__builtin_ldexpf(v[0], ex), __builtin_ldexpf(v[1], ex), __builtin_ldexpf(v[2], ex),
+                        __builtin_ldexpf(v[3], ex));
+        }
+        if (k0 + u * W < a.KB) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const i32x8 wj = __builtin_shufflevector(wf[u][j][0], wf[u][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
+            if constexpr (sizeof(O) == 4)
+              acc[j] = wide_block(wj, xf, sn[u], sc, acc[j]);
+            else
+              acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wj, xf, acc[j], 0, 0, 0, sn[u], 0, sc);
           }
-          if constexpr (sizeof(O) == 4)
-            acc[i] = wide_block(wf, xf, sn, sc, acc[i]);
-          else
-            acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[i], 0, 0, 0, sn, 0, sc);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) part[w][i][r][g * 4 + c] = acc[i][c];   // [row m][column n]
+      for (int c = 0; c < 4; ++c) part[w][j][r][g * 4 + c] = acc[j][c];   // [row m][column n]
     __syncthreads();
-    for (int o = t; o < RT * 256; o += 512) {
-      const int i = o >> 8, m = (o >> 4) & 15, c = o & 15;
-      float v = part[0][i][m][c];
+    for (int o = t; o < TN * 256; o += 512) {
+      const int j = (o >> 4) % TN, m = (o >> 4) / TN, c = o & 15;
+      float v = part[0][j][m][c];
 #pragma unroll
-      for (int u = 1; u < W; ++u) v += part[u][i][m][c];
-      const int64_t row = m0 + 16 * i + m, n = n0 + c;
+      for (int u = 1; u < W; ++u) v += part[u][j][m][c];
+      const int64_t row = m0 + m, n = n0 + 16 * j + c;
       if (row < hi && n < a.N) {
         if (a.bias && !none) v += a.bias[(int64_t)eb * a.N + n];
         if (a.relu) v = relu_of(v);
@@ -575,7 +601,8 @@ void launch_resident(const LinearArgs& a, hipStream_t st) {
 
 template <class X, class T>
 void launch_resident_k(const LinearArgs& a, hipStream_t st) {
-  using S = TileShape<typename std::conditional<sizeof(T) == 4, Fp8Wide, Fp8>::type, 4, 4, 2, 4>;
+  // (the wide products' registers: half the rows)
+  using S = typename std::conditional<sizeof(T) == 4, TileShape<Fp8Wide, 2, 4, 2, 4>, TileShape<Fp8, 4, 4, 2, 4>>::type;
   if (a.KB == 1) launch_resident<S, X, T, 1>(a, st);
   else launch_resident<S, X, T, 2>(a, st);
 }
@@ -587,18 +614,31 @@ void launch_resident_out(const LinearArgs& a, int out_type, hipStream_t st) {
   else launch_resident_k<X, f16>(a, st);
 }
 
-template <class T, class O, int RT>
+template <class T, class O, int TN>
 void launch_skinny(const LinearArgs& a, hipStream_t st) {
-  const bool vec = aligned16(a.x, a.ldx, sizeof(T)) && a.K % 16 == 0;
-  auto* kern = vec ? skinny_kernel<T, O, RT, true> : skinny_kernel<T, O, RT, false>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(a.N, 16), (unsigned)(a.offsets ? a.E + 1 : 1)), dim3(512), 0, st, a);
+  const bool vec = aligned16(a.x, a.ldx, sizeof(T)) && a.K % (16 / sizeof(T)) == 0;
+  auto* kern = vec ? skinny_kernel<T, O, TN, true> : skinny_kernel<T, O, TN, false>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(a.N, 16 * TN), (unsigned)(a.offsets ? a.E + 1 : 1)), dim3(512), 0, st,
+                     a);
+}
+
+template <class T, class O>
+void launch_skinny_n(const LinearArgs& a, hipStream_t st) {
+  // 16-row tiles with work. Wider workgroups round the activations once for more of the weights and
+  // need fewer starts (64 experts of 1024 x 2048, 96 rows: 24 us with 4 tiles, 34 with 2, 34 with 1; one
+  // row, 16384 x 4096: 14, 19, 21), where there are enough of them (6 experts with a row each: 12, 9, 10;
+  // one row, 8192 x 8192: 20, 18, 19; 16 rows, 4096 x 4096: -, 12, 10).
+  const int64_t tiles = cdiv(a.N, 16) * (a.offsets ? (a.M < a.E ? a.M : a.E) : 1);
+  if (tiles >= 1024) launch_skinny<T, O, 4>(a, st);
+  else if (tiles > 256) launch_skinny<T, O, 2>(a, st);
+  else launch_skinny<T, O, 1>(a, st);
 }
 
 template <class T>
 void launch_skinny_out(const LinearArgs& a, int out_type, hipStream_t st) {
-  if (out_type == NERF_F32) launch_skinny<T, float, 1>(a, st);
-  else if (out_type == NERF_BF16) launch_skinny<T, bf16, 1>(a, st);
-  else launch_skinny<T, f16, 1>(a, st);
+  if (out_type == NERF_F32) launch_skinny_n<T, float>(a, st);
+  else if (out_type == NERF_BF16) launch_skinny_n<T, bf16>(a, st);
+  else launch_skinny_n<T, f16>(a, st);
 }
 
 // Few rows for each weight matrix (16, one matrix operand): the skinny form.

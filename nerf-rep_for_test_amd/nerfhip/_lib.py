@@ -199,6 +199,22 @@ def stream_of(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def enqueue(name: str, t, *args) -> None:
+    """``call`` on the current stream of ``t``'s device (the entry's last argument), with that
+    device the current one."""
+    import torch
+    dev = t.device.index
+    stream = torch._C._cuda_getCurrentRawStream(dev)   # (current_stream() without its object: 2 us less)
+    fn = getattr(_lib or lib(), name)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc, name)
+
+
 def require_gpu(t) -> None:
     if not t.is_cuda:
         raise NerfHipError("nerfhip ops need tensors on a ROCm GPU (got %s); there is no CPU "

@@ -14,8 +14,8 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, fp8
-from ._lib import call, ptr
-from .fp8 import TYPES, on_device_of
+from ._lib import enqueue, ptr
+from .fp8 import TYPES
 
 MAX_EXPERTS, MAX_CHOICES, MAX_GROUPS = 1024, 32, 64
 
@@ -41,8 +41,7 @@ def _route(logits, opts):
     experts = torch.empty((T, k), device=logits.device, dtype=torch.int32)
     if T:
         d = _route_desc(logits, opts, weights, experts)
-        with on_device_of(logits):
-            call("nerf_route", ctypes.addressof(d), _lib.stream_of(logits.device))
+        enqueue("nerf_route", logits, ctypes.addressof(d))
     return weights, experts
 
 
@@ -63,9 +62,7 @@ class _RouteFn(torch.autograd.Function):
         if d.numel():
             dweights = dweights.contiguous()
             r = _route_desc(logits, ctx.opts, None, experts)
-            with on_device_of(logits):
-                call("nerf_route_backward", ctypes.addressof(r), ptr(dweights), ptr(d),
-                     _lib.stream_of(logits.device))
+            enqueue("nerf_route_backward", logits, ctypes.addressof(r), ptr(dweights), ptr(d))
         return d, None
 
 
@@ -136,10 +133,8 @@ def plan(experts, num_experts):
         return Plan(order, position, torch.zeros((E + 1,), device=dev, dtype=torch.int32))
     offsets = torch.empty((E + 1,), device=dev, dtype=torch.int32)
     need = _lib.lib().nerf_expert_plan_workspace(n, E)
-    with on_device_of(experts):
-        ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need else None
-        call("nerf_expert_plan", ptr(experts), n, E, ptr(order), ptr(position), ptr(offsets), ptr(ws), need,
-             _lib.stream_of(dev))
+    ws = torch.empty((need,), device=dev, dtype=torch.uint8) if need else None
+    enqueue("nerf_expert_plan", experts, ptr(experts), n, E, ptr(order), ptr(position), ptr(offsets), ptr(ws), need)
     return Plan(order, position, offsets)
 
 
@@ -175,9 +170,8 @@ def _combine(y, weights, p):
     T, k = p.position.shape
     out = torch.empty((T, y.shape[1]), device=y.device, dtype=y.dtype)
     if out.numel():
-        with on_device_of(y):
-            call("nerf_expert_combine", ptr(y), TYPES[y.dtype], y.shape[0], y.shape[1], ptr(weights), ptr(p.position),
-                 T, k, ptr(out), _lib.stream_of(y.device))
+        enqueue("nerf_expert_combine", y, ptr(y), TYPES[y.dtype], y.shape[0], y.shape[1], ptr(weights),
+                ptr(p.position), T, k, ptr(out))
     return out
 
 
@@ -195,10 +189,8 @@ class _CombineFn(torch.autograd.Function):
         dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
         if y.numel() and weights.numel():
             dout = dout.contiguous()
-            with on_device_of(y):
-                call("nerf_expert_combine_backward", ptr(y), TYPES[y.dtype], y.shape[0], y.shape[1], ptr(weights),
-                     ptr(position), ptr(order), ptr(dout), *position.shape, ptr(dy), ptr(dw),
-                     _lib.stream_of(y.device))
+            enqueue("nerf_expert_combine_backward", y, ptr(y), TYPES[y.dtype], y.shape[0], y.shape[1], ptr(weights),
+                    ptr(position), ptr(order), ptr(dout), *position.shape, ptr(dy), ptr(dw))
         elif dw is not None:
             dw.zero_()   # (rows without columns)
         return dy, dw, None, None, None

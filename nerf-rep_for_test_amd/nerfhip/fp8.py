@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import NerfHipError, call, ptr
+from ._lib import NerfHipError, enqueue, ptr
 
 BLOCK = 128
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # NERF_F32 ..
@@ -31,11 +31,6 @@ class _Fp8Linear(ctypes.Structure):
 
 def _blocks(n):
     return -(-n // BLOCK)
-
-
-def on_device_of(t):
-    """A guard that makes ``t``'s device the current one (kernels go to its streams)."""
-    return torch.cuda.device(t.device)
 
 
 class Fp8Weight:
@@ -83,9 +78,8 @@ def quantize_weight(w):
     E, (N, K) = (w.shape[0] if w.dim() == 3 else 1), w.shape[-2:]
     q = torch.empty((*w.shape[:-1], _blocks(K) * BLOCK), device=w.device, dtype=torch.float8_e4m3fn)
     scale = torch.empty((*w.shape[:-2], _blocks(N), _blocks(K)), device=w.device, dtype=torch.uint8)
-    with on_device_of(w):
-        call("nerf_fp8_quantize_weight", ptr(w), TYPES[w.dtype], w.stride(0) if w.dim() == 3 else 0,
-             w.stride(-2), E, N, K, ptr(q), ptr(scale), _lib.stream_of(w.device))
+    enqueue("nerf_fp8_quantize_weight", w, ptr(w), TYPES[w.dtype], w.stride(0) if w.dim() == 3 else 0, w.stride(-2),
+            E, N, K, ptr(q), ptr(scale))
     return Fp8Weight(q, scale, K)
 
 
@@ -119,9 +113,8 @@ def launch(x, weight, M, order, slots, offsets, bias, relu, out_dtype, who):
     d = _Fp8Linear(ptr(x), x.stride(0), x.shape[0], ptr(order), TYPES[x.dtype], TYPES[out_dtype], slots, E,
                    int(relu), M, N, K, ptr(weight.q), ptr(weight.scale), ptr(offsets), ptr(bias), ptr(out), N)
     need = _lib.lib().nerf_fp8_linear_workspace(M, N, K, E, int(offsets is not None))
-    with on_device_of(x):
-        ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
-        call("nerf_fp8_linear", ctypes.addressof(d), ptr(ws), need, _lib.stream_of(x.device))
+    ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
+    enqueue("nerf_fp8_linear", x, ctypes.addressof(d), ptr(ws), need)
     return out
 
 

@@ -13,9 +13,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import call, ptr
-from .adam import HipAdam
-from .fp8 import TYPES, on_device_of
+from ._lib import enqueue, ptr
+from .fp8 import TYPES
 
 STEPS, EPS = 5, 1e-7
 
@@ -38,10 +37,8 @@ class _Options(ctypes.Structure):
 def _run(groups, options, like):
     arr = (_Group * len(groups))(*groups)
     need = _lib.lib().nerf_muon_workspace(ctypes.addressof(arr), len(groups))
-    with on_device_of(like):
-        ws = torch.empty((need,), device=like.device, dtype=torch.uint8)
-        call("nerf_muon", ctypes.addressof(arr), len(groups), ctypes.addressof(options), ptr(ws), need,
-             _lib.stream_of(like.device))
+    ws = torch.empty((need,), device=like.device, dtype=torch.uint8)
+    enqueue("nerf_muon", like, ctypes.addressof(arr), len(groups), ctypes.addressof(options), ptr(ws), need)
 
 
 def _check_steps(steps):
