@@ -305,8 +305,8 @@ constexpr int kScaleRun = 512;   // blocks of K whose weights' scales are in LDS
 // A stage with its rows' scale words, two of them, and the weights' scale bytes.
 template <class S>
 struct ProductLds {
-  static constexpr int kAll = S::kStage + S::BM * 4;
-  static constexpr size_t kBytes = 2 * kAll + (S::BN / 128 > 0 ? S::BN / 128 : 1) * kScaleRun;
+  static constexpr int kAll = S::kStage + (S::BM > S::NT ? S::BM : S::NT) * 4;
+  static constexpr size_t kBytes = S::NS * kAll + (S::BN / 128 > 0 ? S::BN / 128 : 1) * kScaleRun;
 };
 
 template <class S, class T>
@@ -333,44 +333,48 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
     const int64_t nb0 = n0 / 128;
     const unsigned* s0 = (const unsigned*)uniform((int64_t)(a.s + m0));
     const int rows = (int)(hi - 1 - m0 < S::BM ? hi - 1 - m0 : S::BM);
-    char* bytes = lds + 2 * L::kAll;
+    char* bytes = lds + S::NS * L::kAll;
     const unsigned char* mine = (const unsigned char*)bytes + ((w % S::WC) * 16 * S::TN / 128) * kScaleRun;
-    auto load = [&](int k, bool live) {
-      char* stage = lds + (k & 1) * L::kAll;
-      p.load(stage, k, live);
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(s0 + (int64_t)(k >> 2) * a.M), 0, range_of(live),
-                                                        0x00020000);
-#pragma unroll
-      for (int i = 0; i * S::NT < S::BM; ++i) {
-        const int u = __builtin_amdgcn_readfirstlane(w) * 64 + i * S::NT, r = i * S::NT + t;
-        if (u < S::BM)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(
-              rs, (__attribute__((address_space(3))) void*)(stage + S::kStage + u * 4), 4, (r < rows ? r : rows) * 4, 0,
-              0, 0);
+    constexpr int NS = S::NS, kScaleLoads = (S::BM + S::NT - 1) / S::NT;
+    constexpr int kLoads = S::LA + S::LB + kScaleLoads;   // of one wave for one stage
+    struct Plan {
+      typename TileProduct<S>::Loads l;
+      i32x4 rs;
+      unsigned at;
+    };
+    auto plan = [&](int k) {
+      Plan x;
+      char* stage = lds + (k % NS) * L::kAll;
+      x.l = p.loads(stage, k, k < a.KB);
+      x.rs = make_rsrc(s0 + (int64_t)(k >> 2) * a.M, k < a.KB);
+      x.at = lds_offset(stage) + S::kStage + (unsigned)__builtin_amdgcn_readfirstlane(w * 64) * 4u;
+      return x;
+    };
+    auto load = [&](const Plan& x, int q) {
+      p.load_one(x.l, q);
+      if (q >= S::LA + S::LB) {   // (a wave behind the last row loads into the room after it)
+        const int i = q - S::LA - S::LB, r = i * S::NT + t;
+        load_lds4(x.rs, (r < rows ? r : rows) * 4u, x.at + i * S::NT * 4u);
       }
     };
-    load(0, true);
-    for (int k = 0; k < a.KB; ++k) {
-      if (k % kScaleRun == 0) {
-        if (k) __syncthreads();
-        for (int q = t; q < S::BN / 128 * kScaleRun; q += S::NT) {
-          const int64_t nb = nb0 + q / kScaleRun;
-          const int kb = k + q % kScaleRun;
-          if (kb < a.KB && nb < a.NB) bytes[q] = (char)ws[nb * a.KB + kb];
-        }
-      }
-      stage_ready();
-      const char* stage = lds + (k & 1) * L::kAll;
-      typename TileProduct<S>::Frags f;
-      int sm[S::TM];
-      const int sn = mine[k % kScaleRun];
+    auto chunk = [&](int k, auto part) {
+      const char* stage = lds + (k % NS) * L::kAll;
+      int word[S::TM];   // (read first: they are needed first)
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i) sm[i] = (int)(((const unsigned*)(stage + S::kStage))[p.m(i)] >> (8 * (k & 3)));
-      p.read(f, stage);
-      load(k + 1, k + 1 < a.KB);
-      p.mul(f, sm, sn);
-    }
-    stage_ready();
+      for (int i = 0; i < S::TM; ++i) word[i] = ((const int*)(stage + S::kStage))[p.m(i)];
+      const int sn = mine[k % kScaleRun];
+      p.chunk(stage, stage + S::BM * 128, word, 8 * (k & 3), sn, kLoads, part);
+    };
+    auto scales = [&](int k) {   // the weights' scales of the next run of blocks
+      if (k % kScaleRun != 0 || k >= a.KB) return;
+      if (k) __syncthreads();
+      for (int q = t; q < S::BN / 128 * kScaleRun; q += S::NT) {
+        const int64_t nb = nb0 + q / kScaleRun;
+        const int kb = k + q % kScaleRun;
+        if (kb < a.KB && nb < a.NB) bytes[q] = (char)ws[nb * a.KB + kb];
+      }
+    };
+    tile_steps<S, kLoads>(a.KB, plan, load, chunk, scales);
   }
   float bias[4 * S::TN] = {};
   if (!none) load_bias<S>(a, eb, n0 + p.n(), bias);
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int
   unsigned char* sx = (unsigned char*)rows + 2 * KB * S::BM * 128;          // [2][KB][BM]
   TileProduct<S> p;
   p.init(W, ld, 0, 1, W, ld, 0, a.N);
-  for (int k = 0; k < KB; ++k) p.load_n(lds + k * S::BN * 128, k, true);
+  for (int k = 0; k < KB; ++k) p.load_n(lds + k * S::BN * 128, k);
   int sn[KB];
   float bias[4 * S::TN];
   const int nb = (w % S::WC) * 16 * S::TN / 128;
@@ -451,12 +455,11 @@ __global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int
     p.clear();
 #pragma unroll 1   // (the fragments of one block at a time)
     for (int k = 0; k < KB; ++k) {
-      typename TileProduct<S>::Frags f;
-      int sm[S::TM];
+      int word[S::TM];
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i) sm[i] = smine[k * S::BM + p.m(i)];
-      p.read(f, mine + k * S::BM * 128, lds + k * S::BN * 128);
-      p.mul(f, sm, KB == 1 || k == 0 ? sn[0] : sn[KB - 1]);
+      for (int i = 0; i < S::TM; ++i) word[i] = smine[k * S::BM + p.m(i)];
+      p.chunk(mine + k * S::BM * 128, lds + k * S::BN * 128, word, 0, KB == 1 || k == 0 ? sn[0] : sn[KB - 1], 0,
+              [](int) {});
     }
     store_tile<S, T>(a, p, bias, tile * S::BM, a.M, 0);
   }

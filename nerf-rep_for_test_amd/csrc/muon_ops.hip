@@ -25,8 +25,8 @@ typedef _Float16 f16;
 
 constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleA = 32768.0f, kScaleB = 16384.0f;
-constexpr int kMaxGroups = 16;    // stacks of equal matrices in one launch
-constexpr int kNormBlocks = 256;  // partial sums of one matrix's norm, at most
+constexpr int kMaxGroups = 32;    // stacks of equal matrices in one launch
+constexpr int kNormBlocks = 512;  // partial sums of one matrix's norm, at most
 
 struct Group {
   void* out;           // parameters (FP32) or results, [count] matrices out_stride apart
@@ -71,7 +71,9 @@ __device__ __forceinline__ Work work_of(const Group& g, int i) {
 
 __device__ __forceinline__ int find_group(const Batch& b, int& blk) {
   int k = 0;
-  while (k + 1 < b.count && blk >= b.end[k]) ++k;
+#pragma unroll
+  for (int step = kMaxGroups / 2; step >= 1; step /= 2)   // the first group that ends behind blk
+    if (k + step <= b.count - 1 && blk >= b.end[k + step - 1]) k += step;
   blk -= k ? b.end[k - 1] : 0;
   return k;
 }
@@ -97,25 +99,78 @@ __device__ __forceinline__ float clipped(float g, float clip) {   // (NaN stays)
   return g > clip ? clip : (g < -clip ? -clip : g);
 }
 
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+// W (4 or 1) neighbours from element i on as FP32.
+template <int W>
+__device__ __forceinline__ void load_w(float (&f)[W], const void* p, int type, int64_t i) {
+  if (W == 1) {
+    f[0] = load_any(p, type, i);
+  } else if (type == NERF_F32) {
+    const Vec<float, W> v = *(const Vec<float, W>*)((const float*)p + i);
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = v.v[e];
+  } else if (type == NERF_BF16) {
+    const Vec<bf16, W> v = *(const Vec<bf16, W>*)((const bf16*)p + i);
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = (float)v.v[e];
+  } else {
+    const Vec<f16, W> v = *(const Vec<f16, W>*)((const f16*)p + i);
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = (float)v.v[e];
+  }
+}
+
 // The momentum is advanced and the matrices' squares are summed (64 bits: no overflow, a fixed
-// order).
+// order). 4 runs of W values of a thread are in flight together: bound by HBM.
+template <int W>
+__device__ __forceinline__ double norm_part(const Batch& b, const char* src, float* buf, int64_t n, int part, int parts) {
+  double sum = 0.0;
+  const int64_t step = (int64_t)parts * 256 * W;
+  for (int64_t k0 = ((int64_t)part * 256 + threadIdx.x) * W; k0 < n; k0 += 4 * step) {
+    float v[4][W], m[4][W] = {};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t k = k0 + u * step;
+      if (k < n) {
+        load_w<W>(v[u], src, b.type, k);
+        if (buf) load_w<W>(m[u], buf, NERF_F32, k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t k = k0 + u * step;
+      if (k < n) {
+        Vec<float, W> o;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          float x = clipped(v[u][e], b.clip);
+          if (buf) {
+            o.v[e] = m[u][e] * b.mu + x;
+            x = b.nesterov ? x + b.mu * o.v[e] : o.v[e];
+          }
+          sum += (double)x * x;
+        }
+        if (buf) *(Vec<float, W>*)(buf + k) = o;
+      }
+    }
+  }
+  return sum;
+}
+
 __global__ __launch_bounds__(256) void muon_norm_kernel(const Batch b) {
   int blk = blockIdx.x;
   const Group& g = b.g[find_group(b, blk)];
   const int i = blk / g.norm_blocks, part = blk - i * g.norm_blocks;
   const int64_t n = (int64_t)g.m * g.n;
-  const char* src = (const char*)g.g + i * g.g_stride * (b.type == NERF_F32 ? 4 : 2);
+  const int size = b.type == NERF_F32 ? 4 : 2;
+  const char* src = (const char*)g.g + i * g.g_stride * size;
   float* buf = g.buf ? g.buf + i * n : nullptr;
-  double sum = 0.0;
-  for (int64_t k = (int64_t)part * 256 + threadIdx.x; k < n; k += (int64_t)g.norm_blocks * 256) {
-    float v = clipped(load_any(src, b.type, k), b.clip);
-    if (buf) {
-      const float m = buf[k] * b.mu + v;
-      buf[k] = m;
-      v = b.nesterov ? v + b.mu * m : m;
-    }
-    sum += (double)v * v;
-  }
+  const bool vec = n % 4 == 0 && ((uintptr_t)src % (4 * size) | (uintptr_t)buf % 16) == 0;
+  double sum = vec ? norm_part<4>(b, src, buf, n, part, g.norm_blocks) : norm_part<1>(b, src, buf, n, part, g.norm_blocks);
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   __shared__ double w[4];
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
@@ -143,7 +198,8 @@ __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
   const Group& g = b.g[find_group(b, blk)];
   const int tn = (g.n + 63) / 64, tm = (g.m + 63) / 64;
   const int i = blk / (tm * tn), t = blk - i * tm * tn, m0 = t / tn * 64, n0 = t % tn * 64;
-  double sum = threadIdx.x < g.norm_blocks ? g.norm[(int64_t)i * kNormBlocks + threadIdx.x] : 0.0;
+  double sum = 0.0;
+  for (int k = threadIdx.x; k < g.norm_blocks; k += 256) sum += g.norm[(int64_t)i * kNormBlocks + k];
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -151,16 +207,22 @@ __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
   const int64_t size = (int64_t)g.m * g.n;
   const char* src = (const char*)g.g + i * g.g_stride * (b.type == NERF_F32 ? 4 : 2);
   const float* buf = g.buf ? g.buf + i * size : nullptr;
-  for (int q = threadIdx.x; q < 4096; q += 256) {
-    const int y = q >> 6, x = q & 63;
-    float v = 0.0f;
+  float v[16], mo[16] = {};
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const int y = u * 4 + (threadIdx.x >> 6), x = threadIdx.x & 63;
+    v[u] = 0.0f;
     if (m0 + y < g.m && n0 + x < g.n) {
       const int64_t k = (int64_t)(m0 + y) * g.n + n0 + x;
-      v = clipped(load_any(src, b.type, k), b.clip);
-      if (buf) v = b.nesterov ? v + b.mu * buf[k] : buf[k];
-      v *= inv;
+      v[u] = load_any(src, b.type, k);
+      if (buf) mo[u] = buf[k];
     }
-    tile[y][x] = v;
+  }
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    float x = clipped(v[u], b.clip);
+    if (buf) x = b.nesterov ? x + b.mu * mo[u] : mo[u];
+    tile[u * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = x * inv;
   }
   __syncthreads();
   const Work w = work_of(g, i);
@@ -182,6 +244,30 @@ __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
       for (int e = 0; e < 8; ++e) v[e] = split(tile[k + e][row]);
       put8(tra + (n0 + row) * ln, m0 + k, v);
     }
+  }
+}
+
+// 8 neighbours of the result (room: how many exist): the step on the parameters, or X itself.
+template <class T>
+__device__ __forceinline__ void finish(T* at, const float (&f)[8], int room, bool update, float keep, float rate) {
+  constexpr int W = 16 / sizeof(T);
+  if (room >= 8 && (uintptr_t)at % 16 == 0) {
+    Vec<T, W> o[8 / W];
+    if (update) {
+#pragma unroll
+      for (int h = 0; h < 8 / W; ++h) o[h] = *(const Vec<T, W>*)(at + h * W);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      T& v = o[e / W].v[e % W];
+      v = update ? (T)((float)v * keep - f[e] * rate) : (T)f[e];
+    }
+#pragma unroll
+    for (int h = 0; h < 8 / W; ++h) *(Vec<T, W>*)(at + h * W) = o[h];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < room) at[e] = update ? (T)((float)at[e] * keep - f[e] * rate) : (T)f[e];
   }
 }
 
@@ -217,24 +303,26 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
   const int m0 = mt * S::BM, n0 = nt * S::BN, steps = (kdim + 31) / 32;
   TileProduct<S> p;
   p.init(M, ld, m0, rows, N, ld, n0, cols);
-  p.load(lds, 0, true);
-  for (int k = 0; k < steps; ++k) {
-    stage_ready();
-    typename TileProduct<S>::Frags f;
-    p.read(f, lds + (k & 1) * S::kStage);
-    p.load(lds + ((k + 1) & 1) * S::kStage, k + 1, k + 1 < steps);
-    p.mul(f);
-  }
+  using P = TileProduct<S>;
+  constexpr int kLoads = S::LA + S::LB;
+  tile_steps<S, kLoads>(
+      steps, [&](int k) { return p.loads(lds + k % S::NS * S::kStage, k, k < steps); },
+      [&](const typename P::Loads& l, int q) { p.load_one(l, q); },
+      [&](int k, auto part) {
+        const char* stage = lds + k % S::NS * S::kStage;
+        p.chunk(stage, stage + S::BM * 128, kLoads, part);
+      },
+      [](int) {});
   // this lane's rows m, columns n .. n + 4 TN
   const int n = n0 + p.n();
   char* to = STEP == kStepA ? w.a : (STEP == kStepB ? w.b : w.xs);
   const char* add = STEP == kStepB ? w.a : w.xs;   // the term beside the product
   const int64_t lto = row_bytes(cols);
-  constexpr int P = S::BM + 4;   // LDS row of the transposed tile, words
+  constexpr int PITCH = S::BM + 4;   // LDS row of the transposed tile, words
   unsigned* tr = (unsigned*)lds;
-  stage_ready();
   const float unscale = STEP == kStepA ? kScaleA / (g.s * g.s) : 1.0f;
   const float lr = STEP == kStepLast ? (bt.lr_dev ? *bt.lr_dev : bt.lr) : 0.0f;
+  const float keep = 1.0f - lr * bt.decay, rate = lr * g.adjust;
   const bool tall = g.m > g.n;
 #pragma unroll
   for (int q = 0; q < TM; ++q) {
@@ -266,21 +354,15 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
         for (int e = 0; e < 8; ++e) f[e] *= 1.0f / g.s;
         if (tall) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tr[(p.n() + h + e) * P + ml] = __float_as_uint(f[e]);
+          for (int e = 0; e < 8; ++e) tr[(p.n() + h + e) * PITCH + ml] = __float_as_uint(f[e]);
         } else if (m < rows) {
-          T* at = (T*)g.out + i * g.out_stride + (int64_t)m * g.n + nn;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (nn + e < cols) {
-              if (g.buf) at[e] = (T)((float)at[e] * (1.0f - lr * bt.decay) - f[e] * (lr * g.adjust));
-              else at[e] = (T)f[e];
-            }
+          finish<T>((T*)g.out + i * g.out_stride + (int64_t)m * g.n + nn, f, cols - nn, g.buf != nullptr, keep, rate);
         }
       } else {
         if (m < rows && nn < ((cols + 31) & ~31)) put8(to + m * lto, nn, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          tr[(p.n() + h + e) * P + ml] =
+          tr[(p.n() + h + e) * PITCH + ml] =
               (unsigned)__builtin_bit_cast(unsigned short, v[e].hi) | (unsigned)__builtin_bit_cast(unsigned short, v[e].lo) << 16;
       }
     }
@@ -294,16 +376,12 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
   for (int q = threadIdx.x; q < S::BN * S::BM / 8; q += S::NT) {
     const int nl = q / (S::BM / 8), k = q % (S::BM / 8) * 8, nn = n0 + nl, m = m0 + k;
     if (nn >= cols || m >= ((rows + 31) & ~31)) continue;
-    const unsigned* at = tr + nl * P + k;
+    const unsigned* at = tr + nl * PITCH + k;
     if (STEP == kStepLast) {
-      T* o = (T*)g.out + i * g.out_stride + (int64_t)nn * g.n + m;
+      float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (m + e < rows) {
-          const float x = __uint_as_float(at[e]);
-          if (g.buf) o[e] = (T)((float)o[e] * (1.0f - lr * bt.decay) - x * (lr * g.adjust));
-          else o[e] = (T)x;
-        }
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(at[e]);
+      finish<T>((T*)g.out + i * g.out_stride + (int64_t)nn * g.n + m, f, rows - m, g.buf != nullptr, keep, rate);
     } else {
       HiLo v[8];
 #pragma unroll
@@ -339,7 +417,7 @@ int64_t count_tiles(const Group& g, int bm, int bn, bool square) {
 
 template <class S>
 constexpr size_t lds_bytes() {
-  const size_t a = 2 * S::kStage, b = (size_t)S::BN * (S::BM + 4) * 4;
+  const size_t a = S::NS * S::kStage, b = (size_t)S::BN * (S::BM + 4) * 4;
   return a > b ? a : b;
 }
 
@@ -351,7 +429,8 @@ int launch_step(Batch& b, int flip, hipStream_t st) {
     NERF_REQUIRE(end < (1ll << 31), "nerf_muon: too many tiles");
     b.end[k] = (int)end;
   }
-  hipLaunchKernelGGL((muon_product_kernel<S, STEP, T>), dim3((unsigned)end), dim3(S::NT), lds_bytes<S>(), st, b, flip);
+  hipLaunchKernelGGL((muon_product_kernel<S, STEP, T>), dim3((unsigned)end), dim3(S::NT), lds_bytes<S>(),
+                     st, b, flip);
   return check_launch("nerf_muon");
 }
 

@@ -13,11 +13,14 @@
 // A lane's two 16-byte pieces of a chunk (piece g and g + 4, g = lane / 16) are
 // then the whole operand of either form, so staging and reading are the same.
 //
-// Staging: buffer loads into LDS (16 B per lane, no VGPRs) into two LDS stages; the
-// next stage's loads are issued after this stage's fragment reads (the compiler
-// waits for every outstanding LDS load before an LDS read) and land under its
-// MFMAs. Piece p of row r lies at p ^ swz(r), so the 16 rows that a fragment
-// read touches fall into the 16 different 16-byte slots of the 64 banks.
+// Staging: buffer loads straight into LDS (16 B per lane, no VGPRs), S::NS stages. They
+// are issued by inline assembly: the compiler, which cannot tell the stages apart, would
+// make every LDS read wait for all of them, while here a step waits for its own stage
+// only (stage_ready) and the loads of the next NS - 1 stages stay in flight. They write
+// no registers. Counts that the compiler takes of its own loads remain right: more loads
+// in flight only make its waits longer.
+// Piece p of row r lies at p ^ swz(r), so the 16 rows that a fragment read touches fall
+// into the 16 different 16-byte slots of the 64 banks.
 #pragma once
 
 #include <type_traits>
@@ -68,14 +71,38 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// A buffer's range: everything, or nothing. (Opaque to the compiler, which would branch over the
-// loads otherwise.)
-__device__ __forceinline__ int range_of(bool live) { return __builtin_amdgcn_readfirstlane(live ? -1 : 0); }
+// 16 or 4 bytes of each lane, at base + voff, to LDS at lds + 16 (4) lane: `rsrc` as make_rsrc gives it.
+__device__ __forceinline__ void load_lds16(i32x4 rsrc, unsigned voff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds4(i32x4 rsrc, unsigned voff, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc)
+               : "memory", "m0");
+}
+// A buffer from `base` (the same in all lanes) on: everything, or (live false) an empty range, whose
+// loads give zeros.
+__device__ __forceinline__ i32x4 make_rsrc(const void* base, bool live) {
+  const uint64_t b = (uint64_t)base;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)b);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((b >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane(live ? -1 : 0);
+  r[3] = 0x00020000;
+  // (a vector instruction's scalar result needs 5 cycles before a load reads it; the compiler keeps
+  // them for its own loads only)
+  asm volatile("s_nop 4" ::"s"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned lds_offset(const void* p) {
+  return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
 
-// TM x TN tiles of 16 x 16 per wave, WR x WC waves.
-template <class MODE, int TM_, int TN_, int WR_, int WC_>
+// TM x TN tiles of 16 x 16 per wave, WR x WC waves, NS stages.
+template <class MODE, int TM_, int TN_, int WR_, int WC_, int NS_ = 2>
 struct TileShape {
   using Mode = MODE;
+  static constexpr int NS = NS_;
   static constexpr int TM = TM_, TN = TN_, WR = WR_, WC = WC_;
   static constexpr int BM = 16 * TM * WR, BN = 16 * TN * WC, NT = 64 * WR * WC;
   static constexpr int kStage = (BM + BN) * 128;   // bytes of one stage
@@ -138,59 +165,46 @@ struct TileProduct {
     }
   }
 
-  // Starts the loads of chunk k of an operand (M's rows, N's rows) into LDS. `live` false: nothing
-  // is read (an empty range: zeros arrive), so that a loop's last step needs no branch around its
-  // loads; wait for them all the same before the LDS is used again or the wave ends.
-  __device__ __forceinline__ void load_m(char* to, int k, bool live) const { pieces<S::LA>(a0, va, to, k, live); }
-  __device__ __forceinline__ void load_n(char* to, int k, bool live) const { pieces<S::LB>(b0, vb, to, k, live); }
-  __device__ __forceinline__ void load(char* stage, int k, bool live) const {
-    load_m(stage, k, live);
-    load_n(stage + S::BM * 128, k, live);
+  // The loads of chunk k of both operands into a stage, S::LA + S::LB in each wave, one at a time.
+  // `live` false: nothing is read (an empty range: zeros arrive), so that a loop's last steps need no
+  // branch around their loads; wait for them all the same before the LDS is used again or the wave ends.
+  struct Loads {
+    i32x4 ra, rb;
+    unsigned at;
+  };
+  __device__ __forceinline__ Loads loads(char* stage, int k, bool live) const {
+    Loads l;
+    l.at = lds_offset(stage) + (unsigned)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024u;
+    l.ra = make_rsrc(a0 + (int64_t)k * 128, live);
+    l.rb = make_rsrc(b0 + (int64_t)k * 128, live);
+    return l;
   }
-  template <int L>
-  static __device__ __forceinline__ void pieces(const char* base, const unsigned (&v)[L], char* to, int k, bool live) {
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)k * 128), 0, range_of(live), 0x00020000);
+  __device__ __forceinline__ void load_one(const Loads& l, int q) const {
+    if (q < S::LA) load_lds16(l.ra, va[q < S::LA ? q : 0], l.at + q * S::NT * 16);
+    else if (q < S::LA + S::LB) load_lds16(l.rb, vb[q < S::LA ? 0 : q - S::LA], l.at + S::BM * 128 + (q - S::LA) * S::NT * 16);
+  }
+  // Chunk k of B alone, at once.
+  __device__ __forceinline__ void load_n(char* to, int k) const {
+    const Loads l = loads(to - S::BM * 128, k, true);
 #pragma unroll
-    for (int i = 0; i < L; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          r, (__attribute__((address_space(3))) void*)(to + (i * S::NT + w * 64) * 16), 16, (int)v[i], 0, 0, 0);
+    for (int q = 0; q < S::LB; ++q) load_one(l, S::LA + q);
   }
 
   struct Frags {
     i32x4 m[TM][2], n[TN][2];
   };
-  __device__ __forceinline__ void read(Frags& f, const char* stage) const { read(f, stage, stage + S::BM * 128); }
-  __device__ __forceinline__ void read(Frags& f, const char* sa, const char* sb) const {
+  // N tile d and M tile d of a chunk.
+  __device__ __forceinline__ void read(Frags& f, const char* sa, const char* sb, int d) const {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, a = lane & 15;
-    const int wr = (w / S::WC) * 16 * TM, wc = (w % S::WC) * 16 * TN;
-    // one N and one M tile in turn: the first products need only the first of each
-#pragma unroll
-    for (int d = 0; d < (TM > TN ? TM : TN); ++d) {
-      if (d < TN) {
-        const int r = wc + tile_row<TN>(d, a);
-        f.n[d][0] = *(const i32x4*)(sb + r * 128 + ((g ^ swz<TN>(r)) << 4));
-        f.n[d][1] = *(const i32x4*)(sb + r * 128 + (((g + 4) ^ swz<TN>(r)) << 4));
-      }
-      if (d < TM) {
-        const int r = wr + tile_row<TM>(d, a);
-        f.m[d][0] = *(const i32x4*)(sa + r * 128 + ((g ^ swz<TM>(r)) << 4));
-        f.m[d][1] = *(const i32x4*)(sa + r * 128 + (((g + 4) ^ swz<TM>(r)) << 4));
-      }
+    if (d < TN) {
+      const int r = (w % S::WC) * 16 * TN + tile_row<TN>(d, a);
+      f.n[d][0] = *(const i32x4*)(sb + r * 128 + ((g ^ swz<TN>(r)) << 4));
+      f.n[d][1] = *(const i32x4*)(sb + r * 128 + (((g + 4) ^ swz<TN>(r)) << 4));
     }
-  }
-
-  // The products in growing squares (i, j <= d), as their operands arrive.
-  template <class F>
-  static __device__ __forceinline__ void squares(F f) {
-#pragma unroll
-    for (int d = 0; d < (TM > TN ? TM : TN); ++d) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-        if (j < d && d < TM) f(d, j);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-        if (i <= d && d < TN) f(i, d);
+    if (d < TM) {
+      const int r = (w / S::WC) * 16 * TM + tile_row<TM>(d, a);
+      f.m[d][0] = *(const i32x4*)(sa + r * 128 + ((g ^ swz<TM>(r)) << 4));
+      f.m[d][1] = *(const i32x4*)(sa + r * 128 + (((g + 4) ^ swz<TM>(r)) << 4));
     }
   }
 
@@ -198,19 +212,68 @@ struct TileProduct {
     return __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
 
-  // Fp8, Fp8Wide: sm[i] / sn: the rows' scales in the lowest byte (E8M0).
-  __device__ __forceinline__ void mul(const Frags& f, const int (&sm)[TM], int sn) {
-    squares([&](int i, int j) {
-      if constexpr (std::is_same<typename S::Mode, Fp8Wide>::value)
-        acc[i][j] = wide_block(join(f.n[j]), join(f.m[i]), sn & 255, sm[i] & 255, acc[i][j]);
-      else
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(f.n[j]), join(f.m[i]), acc[i][j], 0, 0, 0,
-                                                                     sn, 0, sm[i]);
-    });
+  // One chunk's products, from its rows in LDS, in growing squares (tiles i, j <= d), with part(0) ..
+  // part(parts - 1), the next chunks' loads, along the way.
+  // Large wave tiles (one wave on a SIMD): the operands of square d + 2 are read ahead of square d, so
+  // that the first products wait for the first operands only, and the loads are spread evenly (issued
+  // together they hold up the wave for as long as the memory path takes their addresses). Small ones:
+  // other workgroups cover all that, and the loads are wanted early. 8192 x 8192 x 8192 in 8 bits with
+  // 8 x 8 tiles a wave: 484 us spread, 549 together; 32768 rows of 2048 over 32 experts with 4 x 4: 246 and 226.
+  template <class F, class P>
+  __device__ __forceinline__ void squares(const char* sa, const char* sb, F f, int parts, P part) {
+    constexpr int D = TM > TN ? TM : TN;
+    constexpr bool kLarge = TM * TN > 16;
+    Frags x;
+    int done = 0, at = 0;
+    if (!kLarge) {
+#pragma unroll
+      for (; at < parts; ++at) part(at);
+    }
+    auto one = [&](int i, int j) {
+      f(x, i, j);
+      ++done;
+      bool any = false;
+#pragma unroll
+      for (; at * TM * TN < done * parts; ++at) {
+        part(at);
+        any = true;
+      }
+      if (any) __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int d = 0; d < (kLarge ? 2 : D); ++d) read(x, sa, sb, d);
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (kLarge) {
+        if (d + 2 < D) read(x, sa, sb, d + 2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        if (j < d && d < TM) one(d, j);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+        if (i <= d && d < TN) one(i, d);
+    }
   }
 
-  __device__ __forceinline__ void mul(const Frags& f) {
-    squares([&](int i, int j) {
+  // Fp8, Fp8Wide: word[i] >> shift / sn: the rows' scales in the lowest byte (E8M0).
+  template <class P>
+  __device__ __forceinline__ void chunk(const char* sa, const char* sb, const int (&word)[TM], int shift, int sn, int parts,
+                                        P part) {
+    squares(sa, sb, [&](const Frags& f, int i, int j) {
+      const int sm = (int)((unsigned)word[i] >> shift);
+      if constexpr (std::is_same<typename S::Mode, Fp8Wide>::value)
+        acc[i][j] = wide_block(join(f.n[j]), join(f.m[i]), sn & 255, sm & 255, acc[i][j]);
+      else
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join(f.n[j]), join(f.m[i]), acc[i][j], 0, 0, 0,
+                                                                     sn, 0, sm);
+    }, parts, part);
+  }
+
+  template <class P>
+  __device__ __forceinline__ void chunk(const char* sa, const char* sb, int parts, P part) {
+    squares(sa, sb, [&](const Frags& f, int i, int j) {
       const f16x8 mh = __builtin_bit_cast(f16x8, f.m[i][0]), ml = __builtin_bit_cast(f16x8, f.m[i][1]);
       const f16x8 nh = __builtin_bit_cast(f16x8, f.n[j][0]), nl = __builtin_bit_cast(f16x8, f.n[j][1]);
       f32x4 c = acc[i][j];
@@ -218,7 +281,7 @@ struct TileProduct {
       c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nl, mh, c, 0, 0, 0);
       c = __builtin_amdgcn_mfma_f32_16x16x32_f16(nh, ml, c, 0, 0, 0);
       acc[i][j] = c;
-    });
+    }, parts, part);
   }
 
   // This lane's result rows and columns within the workgroup's tile: tile i -> row m(i),
@@ -233,10 +296,35 @@ struct TileProduct {
   }
 };
 
-// Every wave's outstanding loads have landed and every wave is here.
+// Every wave's loads but the last LEFT have landed, its LDS accesses are done, and every wave is here.
+template <int LEFT = 0>
 __device__ __forceinline__ void stage_ready() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  static_assert(LEFT < 64, "the counter's range");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(LEFT) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The steps k = 0 .. n of a product over S::NS stages. plan(k): what the loads of chunk k into stage
+// k % NS need (nothing that counts behind the last chunk); load(plan, q): one of them, q = 0 .. kLoads - 1 in
+// each wave; chunk(k, part): its products, with part(0) .. part(kLoads - 1) between them. before(k) runs
+// ahead of the barrier behind which chunk k is in LDS.
+template <class S, int kLoads, class PLAN, class LOAD, class CHUNK, class BEFORE>
+__device__ __forceinline__ void tile_steps(int n, PLAN plan, LOAD load, CHUNK chunk, BEFORE before) {
+  constexpr int NS = S::NS;
+#pragma unroll
+  for (int k = 0; k < NS - 1; ++k) {
+    const auto l = plan(k);
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) load(l, q);
+  }
+  for (int k = 0; k < n; ++k) {
+    before(k);
+    const auto l = plan(k + NS - 1);
+    stage_ready<(NS - 2) * kLoads>();
+    chunk(k, [&](int q) { load(l, q); });
+  }
+  stage_ready();   // (nothing is on its way into LDS any more)
 }
 
 // Workgroup p of `total` -> the tile it takes: workgroups go round-robin over the 8 XCDs, so

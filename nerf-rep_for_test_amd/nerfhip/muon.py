@@ -3,7 +3,7 @@
 
 ``orthogonalize`` is the operator alone, ``muon_update`` one step of momentum,
 orthogonalisation, weight decay and step for a list of matrices (17 launches for
-all of them, at most 16 shapes or stacks a set), ``HipMuon`` the optimizer that
+all of them, at most 32 a set), ``HipMuon`` the optimizer that
 the trainer takes: matrices of hidden layers by Muon, everything else by Adam.
 """
 from __future__ import annotations
