@@ -102,13 +102,13 @@ __device__ __forceinline__ int64_t source_row(const int* order, int div, int64_t
   return s < 0 || s / div >= rows ? -1 : s / div;
 }
 
-// Rows of x to e4m3 q [M][KB * 128] and packed scales s [ceil(KB / 4)][M] (the bytes of 4
+// Rows of x (row m: source_row, zeros from `live` on) to e4m3 q [M][KB * 128] and packed scales s [ceil(KB / 4)][M] (the bytes of 4
 // neighbouring blocks of one row in one word). 16 lanes take one block of 128: 8 values
 // each, the largest magnitude by 4 steps inside the 16 lanes. Bound by HBM: every byte
 // is read and written once.
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t ldx, const int* __restrict__ order,
-                                                       int div, int64_t rows, int64_t M, int64_t K, int KB,
+                                                       int div, int64_t rows, int64_t live, int64_t M, int64_t K, int KB,
                                                        unsigned char* __restrict__ q,
                                                        unsigned char* __restrict__ s) {
   const int l = threadIdx.x & 15;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
   for (int64_t b = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); b < blocks; b += (int64_t)gridDim.x * 16) {
     const int64_t m = b / KB;
     const int kb = (int)(b - m * KB);
-    const int64_t src = source_row(order, div, rows, m);
+    const int64_t src = m < live ? source_row(order, div, rows, m) : -1;
     float f[8] = {};
     if (src >= 0) load_row<T, 8, VEC>(f, x + src * ldx, (int64_t)kb * 128 + l * 8, K);
     unsigned top = 0;
@@ -185,8 +185,10 @@ struct LinearArgs {
   int64_t ldx, x_rows;
   const int* order;           // or null
   int div;
-  const unsigned char* q;     // quantised rows [M][KB * 128] (tiled form)
-  const unsigned* s;          // [ceil(KB / 4)][M]
+  const unsigned char* q;     // quantised rows [q_rows][KB * 128] (tiled form)
+  const unsigned* s;          // [ceil(KB / 4)][q_rows]
+  int64_t q_rows;
+  int gather;                 // q holds x's rows and one of zeros; else the M rows as they are taken
   const unsigned char* wq;    // [E][N][KB * 128]
   const unsigned char* ws;    // [E][NB][KB]
   const int* offsets;         // [E + 1], or null (dense: E = 1)
@@ -324,19 +326,30 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
   const bool none = e == a.E && a.offsets;
   const int64_t ld = (int64_t)a.KB * 128;
   const int eb = none ? 0 : e;
-  p.init((const char*)a.q, ld, m0, hi, (const char*)a.wq + (int64_t)eb * a.N * ld, ld, n0, a.N);
+  // a tile's rows among the quantised ones: neighbours, or x's rows where `order` says (the row of zeros
+  // behind them for none)
+  const int64_t first = a.gather ? 0 : m0;
+  const auto row = [&](int r) {
+    const int64_t m = m0 + r < hi ? m0 + r : hi - 1;
+    if (!a.gather) return (unsigned)(m - m0);
+    const int64_t src = source_row(a.order, a.div, a.x_rows, m);
+    return (unsigned)(src < 0 ? a.x_rows : src);
+  };
+  p.init_rows((const char*)a.q + first * ld, (unsigned)ld, row, (const char*)a.wq + (int64_t)eb * a.N * ld, ld, n0, a.N);
   if (!none) {
     // Scales reach the loop through LDS only, so nothing in it waits for a load into registers:
     // the rows' words (4 blocks) with each stage, the weights' bytes kScaleRun blocks at a time.
     const int t = threadIdx.x, w = t >> 6;
     const unsigned char* ws = a.ws + (int64_t)eb * a.NB * a.KB;
     const int64_t nb0 = n0 / 128;
-    const unsigned* s0 = (const unsigned*)uniform((int64_t)(a.s + m0));
-    const int rows = (int)(hi - 1 - m0 < S::BM ? hi - 1 - m0 : S::BM);
+    const unsigned* s0 = (const unsigned*)uniform((int64_t)(a.s + first));
     char* bytes = lds + S::NS * L::kAll;
     const unsigned char* mine = (const unsigned char*)bytes + ((w % S::WC) * 16 * S::TN / 128) * kScaleRun;
     constexpr int NS = S::NS, kScaleLoads = (S::BM + S::NT - 1) / S::NT;
     constexpr int kLoads = S::LA + S::LB + kScaleLoads;   // of one wave for one stage
+    unsigned srow[kScaleLoads];
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) srow[i] = row(i * S::NT + t) * 4u;
     struct Plan {
       typename TileProduct<S>::Loads l;
       i32x4 rs;
@@ -346,15 +359,15 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
       Plan x;
       char* stage = lds + (k % NS) * L::kAll;
       x.l = p.loads(stage, k, k < a.KB);
-      x.rs = make_rsrc(s0 + (int64_t)(k >> 2) * a.M, k < a.KB);
+      x.rs = make_rsrc(s0 + (int64_t)(k >> 2) * a.q_rows, k < a.KB);
       x.at = lds_offset(stage) + S::kStage + (unsigned)__builtin_amdgcn_readfirstlane(w * 64) * 4u;
       return x;
     };
     auto load = [&](const Plan& x, int q) {
       p.load_one(x.l, q);
       if (q >= S::LA + S::LB) {   // (a wave behind the last row loads into the room after it)
-        const int i = q - S::LA - S::LB, r = i * S::NT + t;
-        load_lds4(x.rs, (r < rows ? r : rows) * 4u, x.at + i * S::NT * 4u);
+        const int i = q - S::LA - S::LB;
+        load_lds4(x.rs, srow[i], x.at + i * S::NT * 4u);
       }
     };
     auto chunk = [&](int k, auto part) {
@@ -578,13 +591,13 @@ bool aligned16(const void* p, int64_t ld, int size) {
 }
 
 template <class T>
-void launch_quantize(const NerfFp8Linear* d, int KB, unsigned char* q, unsigned char* s, hipStream_t st) {
-  const int64_t groups = cdiv(d->M * KB, 16);
+void launch_quantize(const LinearArgs& a, unsigned char* q, unsigned char* s, hipStream_t st) {
+  const int64_t groups = cdiv(a.q_rows * a.KB, 16);
   const unsigned grid = (unsigned)(groups < 65536 ? groups : 65536);
-  const bool vec = aligned16(d->x, d->ldx, sizeof(T)) && d->K % (16 / sizeof(T)) == 0;
+  const bool vec = aligned16(a.x, a.ldx, sizeof(T)) && a.K % (16 / sizeof(T)) == 0;
   auto* kern = vec ? quantize_kernel<T, true> : quantize_kernel<T, false>;
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, st, (const T*)d->x, d->ldx, d->order, d->order ? d->slots : 1,
-                     d->x_rows, d->M, d->K, KB, q, s);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, st, (const T*)a.x, a.ldx, a.gather ? nullptr : a.order, a.div, a.x_rows,
+                     a.gather ? a.x_rows : a.q_rows, a.q_rows, a.K, a.KB, q, s);
 }
 
 template <class S, class T>
@@ -676,7 +689,7 @@ extern "C" {
 size_t nerf_fp8_linear_workspace(int64_t M, int64_t N, int64_t K, int E, int grouped) {
   if (M < 1 || N < 1 || K < 1 || is_skinny(M, E, grouped != 0) || is_resident(M, N, K, grouped != 0)) return 0;
   const int64_t KB = cdiv(K, 128);
-  return (size_t)(M * KB * 128 + cdiv(KB, 4) * M * 4);
+  return (size_t)((M + 1) * KB * 128 + cdiv(KB, 4) * (M + 1) * 4);   // (a row of zeros behind the others)
 }
 
 int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_bytes, nerf_stream_t stream) {
@@ -703,6 +716,8 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   a.ldo = d->ldo;
   a.q = nullptr;
   a.s = nullptr;
+  a.q_rows = 0;
+  a.gather = 0;
   if (is_skinny(d->M, d->E, d->offsets != nullptr)) {
     if (d->x_type == NERF_F32) launch_skinny_out<float>(a, d->out_type, st);
     else if (d->x_type == NERF_BF16) launch_skinny_out<bf16>(a, d->out_type, st);
@@ -719,7 +734,11 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
                    workspace_bytes >= nerf_fp8_linear_workspace(d->M, d->N, d->K, d->E, d->offsets != nullptr),
                "nerf_fp8_linear: workspace too small or unaligned");
   unsigned char* q = (unsigned char*)workspace;
-  unsigned char* s = q + d->M * a.KB * 128;
+  // experts' rows: x is rounded once, not once for each of its slots, and the tiles take its rows where
+  // they are (32-bit offsets)
+  a.gather = d->order && (d->x_rows + 1) * a.KB * 128 < (1ll << 32) && d->x_rows <= d->M;
+  a.q_rows = a.gather ? d->x_rows + 1 : d->M;
+  unsigned char* s = q + a.q_rows * a.KB * 128;
   a.q = q;
   a.s = (const unsigned*)s;
   using S = TileShape<Fp8, 4, 4, 2, 2>;
@@ -730,9 +749,9 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   using SL = TileShape<Fp8, 8, 8, 2, 2>;
   const bool large = d->K >= 4096 && cdiv(d->M, 256) * cdiv(d->N, 256) >= 512;
   NERF_REQUIRE((d->M / S::BM + d->E + 1) * cdiv(d->N, S::BN) < (1ll << 31), "nerf_fp8_linear: too many tiles");
-  if (d->x_type == NERF_F32) launch_quantize<float>(d, a.KB, q, s, st);
-  else if (d->x_type == NERF_BF16) launch_quantize<bf16>(d, a.KB, q, s, st);
-  else launch_quantize<f16>(d, a.KB, q, s, st);
+  if (d->x_type == NERF_F32) launch_quantize<float>(a, q, s, st);
+  else if (d->x_type == NERF_BF16) launch_quantize<bf16>(a, q, s, st);
+  else launch_quantize<f16>(a, q, s, st);
   if (const int rc = check_launch("nerf_fp8_linear")) return rc;
   if (d->out_type == NERF_F32) launch_product<SW, float>(a, st);
   else if (d->out_type == NERF_BF16) large ? launch_product<SL, bf16>(a, st) : launch_product<S, bf16>(a, st);

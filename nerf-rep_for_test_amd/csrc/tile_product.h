@@ -134,13 +134,18 @@ struct TileProduct {
   // again (their results are not stored). lda, ldb: bytes, 2^24 at most.
   __device__ __forceinline__ void init(const char* A, int64_t lda, int64_t m0, int64_t M, const char* B,
                                        int64_t ldb, int64_t n0, int64_t N) {
-    const int t = threadIdx.x;
-    a0 = (const char*)uniform((int64_t)(A + m0 * lda));
     const int am = (int)(M - 1 - m0 < S::BM ? M - 1 - m0 : S::BM);
+    init_rows(A + m0 * lda, (unsigned)lda, [&](int r) { return (unsigned)(r < am ? r : am); }, B, ldb, n0, N);
+  }
+  // Tile row r of A is row row(r) from `base` on (below 4 GiB).
+  template <class ROW>
+  __device__ __forceinline__ void init_rows(const char* base, unsigned lda, ROW row, const char* B, int64_t ldb, int64_t n0,
+                                            int64_t N) {
+    a0 = (const char*)uniform((int64_t)base);
 #pragma unroll
     for (int i = 0; i < S::LA; ++i) {
-      const int idx = i * S::NT + t, r = idx >> 3, p = (idx & 7) ^ swz<TM>(r);
-      va[i] = (unsigned)(r < am ? r : am) * (unsigned)lda + p * 16;
+      const int idx = i * S::NT + (int)threadIdx.x, r = idx >> 3, p = (idx & 7) ^ swz<TM>(r);
+      va[i] = row(r) * lda + p * 16;
     }
     set_n(B, ldb, n0, N);
     clear();

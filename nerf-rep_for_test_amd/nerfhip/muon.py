@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import enqueue, ptr
+from .adam import HipAdam
 from .fp8 import TYPES
 
 STEPS, EPS = 5, 1e-7
@@ -117,3 +118,82 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     o = _Options(0, 1, int(bool(nesterov)), steps, 0.0 if dev_lr else float(lr), float(momentum), float(weight_decay),
                  float(eps), -1.0 if clip is None else float(clip), ptr(lr) if dev_lr else None)
     _run(groups, o, params[0])
+
+
+def is_hidden_matrix(p):
+    """What HipMuon orthogonalises: matrices with 16 rows and columns at least (a network's hidden
+    layers; its density and colour heads have 1 and 3 rows)."""
+    return p.dim() == 2 and min(p.shape) >= 16
+
+
+class HipMuon(torch.optim.Optimizer):
+    """Muon for the matrices that ``is_hidden_matrix`` names, HipAdam (same ``lr``, ``betas``, ``adam_eps``)
+    for every other parameter; gradients clamped to [-``clip``, clip] on their way in (None: not). Matrices
+    move by ``lr * muon_ratio`` times an orthogonal matrix: with Adam's usual 5e-4 and the ratio 40 by 0.02.
+
+    Group 0 holds the matrices (state: ``momentum_buffer``), group 1 the rest (HipAdam's state). lr is a
+    device tensor in both (fill it to change it; the step then stays one captured graph). float32 contiguous
+    parameters on one ROCm device; every parameter needs a gradient at every step, as with HipAdam."""
+
+    def __init__(self, params, lr=5e-4, muon_ratio=40.0, momentum=0.95, nesterov=True, weight_decay=0.0, steps=STEPS,
+                 betas=(0.9, 0.999), adam_eps=1e-8, clip=None):
+        params = list(params)
+        if any(isinstance(p, dict) for p in params):
+            raise ValueError("HipMuon takes parameters, not groups: it makes its own two")
+        matrices = [p for p in params if is_hidden_matrix(p)]
+        rest = [p for p in params if not is_hidden_matrix(p)]
+        if not matrices:
+            raise ValueError("HipMuon: no matrix with 16 rows and columns among the parameters")
+        if not muon_ratio > 0:
+            raise ValueError("HipMuon: muon_ratio must be positive")
+        if clip is not None and not clip >= 0:
+            raise ValueError("HipMuon: clip must be None (no clipping) or >= 0")
+        dev = matrices[0].device
+        if dev.type != "cuda":
+            raise _lib.NerfHipError("HipMuon needs a ROCm GPU device (no CPU fallback)")
+        self.adam = HipAdam(rest, lr=lr, betas=betas, eps=adam_eps, clip=clip) if rest else None
+        self.muon_ratio, self.clip = float(muon_ratio), clip
+        self._lr = torch.zeros((), device=dev, dtype=torch.float32)
+        super().__init__([{"params": matrices}],
+                         dict(lr=torch.tensor(lr, device=dev, dtype=torch.float32), momentum=float(momentum),
+                              nesterov=bool(nesterov), weight_decay=float(weight_decay), steps=_check_steps(steps)))
+        if self.adam is not None:
+            self.param_groups.append(self.adam.param_groups[0])
+            self._share()
+
+    def _share(self):
+        """One state and one group object for both optimizers."""
+        if self.adam is not None:
+            self.adam.state = self.state
+            self.adam.param_groups = [self.param_groups[1]]
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        self._share()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        if closure is not None:
+            raise ValueError("HipMuon.step takes no closure")
+        g = self.param_groups[0]
+        missing = [p for h in self.param_groups for p in h["params"] if p.grad is None]
+        every = sum(len(h["params"]) for h in self.param_groups)
+        if missing:
+            if len(missing) == every:
+                return None
+            raise ValueError(f"HipMuon: {len(missing)} of {every} parameters have no gradient")
+        lr = g["lr"]
+        if not torch.is_tensor(lr):   # a float lr set by someone else: back on the device
+            lr = g["lr"] = torch.tensor(float(lr), device=self._lr.device)
+        buffers = []
+        for p in g["params"]:
+            st = self.state[p]
+            if "momentum_buffer" not in st:
+                st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+            buffers.append(st["momentum_buffer"])
+        torch.mul(lr, self.muon_ratio, out=self._lr)
+        muon_update(g["params"], [p.grad for p in g["params"]], buffers, self._lr, momentum=g["momentum"],
+                    nesterov=g["nesterov"], weight_decay=g["weight_decay"], steps=g["steps"], clip=self.clip)
+        if self.adam is not None:
+            self.adam.step()
+        return None

@@ -284,14 +284,18 @@ class NerfTrainer:
         # adam: "hip" (the default: clip_grad_value_ + Adam in one nerf_adam_step
         # launch, lr and step count on the device, graph-capturable), or torch's
         # "fused" (eager only) / "capturable" multi-tensor Adam after a separate
-        # clip_grad_value_
+        # clip_grad_value_; "muon": hidden layers' matrices by Muon, the rest by "hip"
+        # (muon.HipMuon: lr is Adam's, the matrices move by 40 lr)
         adam = adam or "hip"
-        if adam not in ("hip", "fused", "capturable") or (self.graph and adam == "fused"):
-            raise ValueError("adam must be 'hip', 'fused' or 'capturable' (graph: not 'fused')")
+        if adam not in ("hip", "fused", "capturable", "muon") or (self.graph and adam == "fused"):
+            raise ValueError("adam must be 'hip', 'fused', 'capturable' or 'muon' (graph: not 'fused')")
         self.adam = adam
         if adam == "hip":
             from .adam import HipAdam
             self.opt = HipAdam(self.trained_parameters(), lr=lr, eps=1e-8, clip=self.clip_value)
+        elif adam == "muon":
+            from .muon import HipMuon
+            self.opt = HipMuon(self.trained_parameters(), lr=lr, clip=self.clip_value)
         elif adam == "capturable":
             self.opt = torch.optim.Adam(self.trained_parameters(),
                                         lr=torch.tensor(lr, device=self.device), eps=1e-8,
@@ -453,7 +457,7 @@ class NerfTrainer:
                 if p.grad is None:   # (a rank whose batch left a parameter untouched):
                     p.grad = torch.zeros_like(p)   # every rank sends the same bucket
             allreduce_mean([p.grad for p in self.trained_parameters()], group)
-        if self.adam != "hip":   # (HipAdam clamps the gradients itself, in place)
+        if self.adam not in ("hip", "muon"):   # (HipAdam and HipMuon clamp the gradients themselves)
             torch.nn.utils.clip_grad_value_(self.trained_parameters(), self.clip_value)
         self.opt.step()
         return losses

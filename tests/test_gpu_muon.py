@@ -5,6 +5,7 @@ L = 4 (3.4445 at 0, 3.97 at the end), so what a step adds to the error is multip
 A step's own error is taken as e |X_k| (Frobenius) with e = 2^-19: operands of 22 bits (2^-22 each, three products
 in a row with coefficients a, b, c: 10 * 2^-22 at most together), the FP32 sums below that. |X_k| <= min(L^k,
 1.2024 sqrt r)."""
+import copy
 import math
 
 import pytest
@@ -182,3 +183,80 @@ def test_update_in_a_graph_and_on_another_stream(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(pg, want[k])), k
         muon.orthogonalize(gs[k][0])
+
+
+def _params(dev, seed=3):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    shapes = [(256, 63), (256,), (256, 256), (1, 256), (1,), (3, 128), (128, 283), (128,), (16, 16), (15, 40)]
+    return [torch.randn(s, device=dev, generator=g).requires_grad_() for s in shapes], g
+
+
+def test_hip_muon_splits_the_parameters(dev):
+    """Matrices as muon_update, the rest bit for bit as HipAdam alone; lr through the device tensor; a state
+    dict round trip goes on as if nothing had been."""
+    from nerfhip.adam import HipAdam
+    from nerfhip.muon import HipMuon, is_hidden_matrix, muon_update
+    pa, g = _params(dev)
+    pb, _ = _params(dev)
+    pc, _ = _params(dev)
+    opt = HipMuon(pa, lr=1e-3, clip=20.0)
+    assert [len(v["params"]) for v in opt.param_groups] == [4, 6]
+    mats, rest = [p for p in pb if is_hidden_matrix(p)], [p for p in pb if not is_hidden_matrix(p)]
+    adam, bufs = HipAdam(rest, lr=1e-3, clip=20.0), [torch.zeros_like(p) for p in mats]
+    for step in range(6):
+        if step == 3:
+            again = HipMuon(pc, lr=5.0, clip=20.0)
+            with torch.no_grad():
+                torch._foreach_copy_(pc, pa)
+            again.load_state_dict(copy.deepcopy(opt.state_dict()))   # (torch's own would share the tensors)
+            for v in opt.param_groups:
+                v["lr"].fill_(4e-4)
+            for v in again.param_groups:
+                v["lr"].fill_(4e-4)
+            adam.param_groups[0]["lr"].fill_(4e-4)
+        lr = torch.tensor(1e-3 if step < 3 else 4e-4, device=dev)
+        for a, b, c in zip(pa, pb, pc):
+            gr = torch.randn(a.shape, device=dev, generator=g) * 15.0
+            a.grad, b.grad, c.grad = gr.clone(), gr.clone(), gr.clone()
+        opt.step()
+        adam.step()
+        muon_update([p.detach() for p in mats], [p.grad for p in mats], bufs, lr * 40.0, clip=20.0)
+        if step >= 3:
+            again.step()
+            assert all(torch.equal(a, c) for a, c in zip(pa, pc)), step
+        assert all(torch.equal(a, b) for a, b in zip(pa, pb)), step
+    pa[0].grad = None
+    with pytest.raises(ValueError, match="no gradient"):
+        opt.step()
+
+
+@pytest.mark.parametrize("n_importance", [128, 0])
+def test_trainer_steps_with_muon(dev, n_importance):
+    """NerfTrainer(adam="muon"): graph steps (two eager, the capture, replays) equal eager ones bit for bit, the
+    matrices move by 40 lr times a nearly orthogonal matrix, and lr 0 moves nothing."""
+    from goldlib import load, params_of
+    from nerfhip.train import NerfTrainer
+    z = load("t1_train_step")
+    g = torch.Generator(device=dev).manual_seed(1)
+    n = 256
+    ro = torch.randn(n, 3, device=dev, generator=g) * 0.1 + torch.tensor([0.0, 0.0, 4.0], device=dev)
+    rd = torch.nn.functional.normalize(torch.randn(n, 3, device=dev, generator=g) * 0.2 -
+                                       torch.tensor([0.0, 0.0, 1.0], device=dev), dim=-1)
+    gt = torch.rand(n, 3, device=dev, generator=g)
+    runs = []
+    for graph in (False, True):
+        torch.manual_seed(5)
+        tr = NerfTrainer(dev, params_of(z), N_importance=n_importance, graph=graph, adam="muon", lr=1e-4)
+        first = {k: v.clone() for k, v in tr.state().items()}
+        losses = [float(tr.step(ro, rd, gt)["loss"]) for _ in range(6)]
+        runs.append((losses, {k: v.clone() for k, v in tr.state().items()}, tr))
+    assert runs[0][0] == runs[1][0]
+    for k, v in runs[0][1].items():
+        assert torch.equal(v, runs[1][1][k]), k
+    tr = runs[1][2]
+    moved = (runs[0][1]["model.pts_linears.2.weight"] - first["model.pts_linears.2.weight"]).norm()
+    assert 0 < float(moved) <= 6 * 40 * 1e-4 * 1.2024 * 16      # six steps of at most 1.2024 sqrt(256)
+    tr.set_lr(0.0)
+    before = [p.detach().clone() for p in tr.trained_parameters()]
+    tr.step(ro, rd, gt)
+    assert all(torch.equal(a, b) for a, b in zip(before, tr.trained_parameters()))
