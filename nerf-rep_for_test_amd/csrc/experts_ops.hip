@@ -845,17 +845,16 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restri
 // ---------------------------------------------------------------- launches
 
 int check_route(const NerfRoute* d, const char* who, bool fwd) {
-  const std::string at(who);
-  if (!d) return fail(NERF_E_ARG, at + ": null pointer");
-  if (!d->logits || !d->experts || (fwd && !d->weights)) return fail(NERF_E_ARG, at + ": null pointer");
-  if (d->T < 1 || d->T >= (1ll << 31) || d->E < 1 || d->E > kMaxExperts || d->ld < 0)
-    return fail(NERF_E_ARG, at + ": bad size (1 to 1024 experts)");
-  if (d->k < 1 || d->k > kMaxChoices || d->k > d->E) return fail(NERF_E_ARG, at + ": k must be 1 to 32, and at most E");
-  if (d->groups < 1 || d->groups > kMaxGroups || d->E % d->groups || d->top_groups < 1 || d->top_groups > d->groups ||
-      (int64_t)d->top_groups * (d->E / d->groups) < d->k)
-    return fail(NERF_E_ARG, at + ": groups must divide E, and top_groups of them hold k experts");
-  if (d->type < NERF_F32 || d->type > NERF_F16) return fail(NERF_E_ARG, at + ": bad type");
-  return 0;
+  const char* why = nullptr;
+  if (!d || !d->logits || !d->experts || (fwd && !d->weights)) why = "null pointer";
+  else if (d->T < 1 || d->T >= (1ll << 31) || d->E < 1 || d->E > kMaxExperts || d->ld < 0)
+    why = "bad size (1 to 1024 experts)";
+  else if (d->k < 1 || d->k > kMaxChoices || d->k > d->E) why = "k must be 1 to 32, and at most E";
+  else if (d->groups < 1 || d->groups > kMaxGroups || d->E % d->groups || d->top_groups < 1 || d->top_groups > d->groups ||
+           (int64_t)d->top_groups * (d->E / d->groups) < d->k)
+    why = "groups must divide E, and top_groups of them hold k experts";
+  else if (d->type < NERF_F32 || d->type > NERF_F16) why = "bad type";
+  return why ? fail(NERF_E_ARG, std::string(who) + ": " + why) : 0;
 }
 
 RouteArgs route_args(const NerfRoute* d) {

@@ -314,7 +314,8 @@ struct ProductLds {
 template <class S, class T>
 __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int mtiles, int ntiles) {
   using L = ProductLds<S>;
-  static_assert(S::BN % 128 == 0 && 128 % (16 * S::TN) == 0 && S::BM % 64 == 0, "one scale for a wave's columns");
+  static_assert(128 % (16 * S::TN) == 0 && (S::BN % 128 == 0 || 128 % S::BN == 0), "one scale for a wave's columns");
+  constexpr int kBlocksN = S::BN > 128 ? S::BN / 128 : 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int64_t id = xcd_tile(blockIdx.x, gridDim.x);
   int e, mt, nt;
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
     const int64_t nb0 = n0 / 128;
     const unsigned* s0 = (const unsigned*)uniform((int64_t)(a.s + first));
     char* bytes = lds + S::NS * L::kAll;
-    const unsigned char* mine = (const unsigned char*)bytes + ((w % S::WC) * 16 * S::TN / 128) * kScaleRun;
+    const unsigned char* mine = (const unsigned char*)bytes + (S::BN > 128 ? (w % S::WC) * 16 * S::TN / 128 : 0) * kScaleRun;
     constexpr int NS = S::NS, kScaleLoads = (S::BM + S::NT - 1) / S::NT;
     constexpr int kLoads = S::LA + S::LB + kScaleLoads;   // of one wave for one stage
     unsigned srow[kScaleLoads];
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
     auto scales = [&](int k) {   // the weights' scales of the next run of blocks
       if (k % kScaleRun != 0 || k >= a.KB) return;
       if (k) __syncthreads();
-      for (int q = t; q < S::BN / 128 * kScaleRun; q += S::NT) {
+      for (int q = t; q < kBlocksN * kScaleRun; q += S::NT) {
         const int64_t nb = nb0 + q / kScaleRun;
         const int kb = k + q % kScaleRun;
         if (kb < a.KB && nb < a.NB) bytes[q] = (char)ws[nb * a.KB + kb];
@@ -657,8 +658,10 @@ void launch_skinny_out(const LinearArgs& a, int out_type, hipStream_t st) {
   else launch_skinny_n<T, f16>(a, st);
 }
 
-// Few rows for each weight matrix (16, one matrix operand): the skinny form.
-bool is_skinny(int64_t M, int E, bool grouped) { return grouped ? M <= 16 * (int64_t)E : M <= 16; }
+// Few rows for each weight matrix: the skinny form, which takes 16 rows (one matrix operand) at a time and
+// reads the weights again for the next 16 (4096 x 4096, 16-bit rows: 32 of them 17 us, tiled 21; 48: 23
+// and 21; 16 experts of 1024 x 2048 with 256 rows: 16 and 18 us, with 512: 23 and 19).
+bool is_skinny(int64_t M, int E, bool grouped) { return grouped ? M <= 16 * (int64_t)E : M <= 32; }
 
 // Many rows through one small matrix: the resident form (a tile for every CU at least).
 bool is_resident(int64_t M, int64_t N, int64_t K, bool grouped) {
@@ -748,12 +751,20 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   // (8192 x 8192 x 8192: 534 us against 591; 32768 rows of 2048 over 32 experts: 269 against 243).
   using SL = TileShape<Fp8, 8, 8, 2, 2>;
   const bool large = d->K >= 4096 && cdiv(d->M, 256) * cdiv(d->N, 256) >= 512;
-  NERF_REQUIRE((d->M / S::BM + d->E + 1) * cdiv(d->N, S::BN) < (1ll << 31), "nerf_fp8_linear: too many tiles");
+  // 64 x 64 where the larger tiles would leave CUs without one.
+  using SS = TileShape<Fp8, 2, 2, 2, 2>;
+  using SWS = TileShape<Fp8Wide, 2, 2, 2, 2>;
+  const bool small = (cdiv(d->M, 128) + (d->offsets ? (d->M < d->E ? d->M : d->E) : 0)) * cdiv(d->N, 128) <= 256;
+  NERF_REQUIRE((d->M / SS::BM + d->E + 1) * cdiv(d->N, SS::BN) < (1ll << 31), "nerf_fp8_linear: too many tiles");
   if (d->x_type == NERF_F32) launch_quantize<float>(a, q, s, st);
   else if (d->x_type == NERF_BF16) launch_quantize<bf16>(a, q, s, st);
   else launch_quantize<f16>(a, q, s, st);
   if (const int rc = check_launch("nerf_fp8_linear")) return rc;
-  if (d->out_type == NERF_F32) launch_product<SW, float>(a, st);
+  if (small) {
+    if (d->out_type == NERF_F32) launch_product<SWS, float>(a, st);
+    else if (d->out_type == NERF_BF16) launch_product<SS, bf16>(a, st);
+    else launch_product<SS, f16>(a, st);
+  } else if (d->out_type == NERF_F32) launch_product<SW, float>(a, st);
   else if (d->out_type == NERF_BF16) large ? launch_product<SL, bf16>(a, st) : launch_product<S, bf16>(a, st);
   else large ? launch_product<SL, f16>(a, st) : launch_product<S, f16>(a, st);
   return check_launch("nerf_fp8_linear");

@@ -124,8 +124,8 @@ def linear(x, weight, bias=None, relu=False, out_dtype=None):
     value that is not finite makes its row's outputs NaN."""
     if not isinstance(weight, Fp8Weight) or weight.q.dim() != 2:
         raise ValueError("linear: weight must be an Fp8Weight of one matrix")
-    if x.dim() < 1:
-        raise ValueError("linear: activations must be [.., K]")
+    if x.dim() < 1 or x.shape[-1] != weight.k:
+        raise ValueError(f"linear: activations must be [.., {weight.k}]")
     flat = x.reshape(-1, x.shape[-1])
     y = launch(flat, weight, flat.shape[0], None, 1, None, bias, relu, out_dtype, "linear")
     return y.view(*x.shape[:-1], y.shape[1])

@@ -79,6 +79,7 @@ def test_products_and_joins_refuse():
         lambda: fp8.linear(x, w),
         lambda: fp8.linear(x, weight(8, 100), bias=torch.zeros(8).half()),
         lambda: fp8.linear(torch.zeros(()), weight(8, 100)),
+        lambda: fp8.linear(torch.zeros(3, 0), weight(8, 100)),
         lambda: fp8.linear(torch.zeros(3, 128), weight(8, 100)),
         lambda: fp8.quantize_weight(torch.zeros(4)),
         lambda: fp8.quantize_weight(torch.zeros(0, 4)),

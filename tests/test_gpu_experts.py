@@ -319,3 +319,53 @@ def test_a_trained_gate_end_to_end(dev):
     rg, rw = torch.autograd.grad((ref ** 2).sum(), [g64, w64])
     for got, want in ((dg, rg), (dws, rw)):
         assert float((got.cpu().double() - want).norm() / want.norm()) < 1e-5
+
+
+def test_a_captured_training_step_replays(dev):
+    """Gate, plan, join and their backward in one graph (torch.autograd.grad), with eager work and
+    synchronisation between the replays, against eager steps."""
+    from nerfhip import experts
+    T, E, k, N = 300, 10, 3, 48
+    logits = [torch.randn(T, E, device=dev) for _ in range(3)]
+    ys = [torch.randn(T * k, N, device=dev).bfloat16() for _ in range(3)]
+    douts = [torch.randn(T, N, device=dev).bfloat16() for _ in range(3)]
+
+    def step(l, y, d):
+        w, e = experts.route(l, k, score="sigmoid", groups=5, top_groups=2)
+        p = experts.plan(e, E)
+        out = experts.combine(y, w, p)
+        return (e, out.detach(), *torch.autograd.grad(out, [l, y], d))
+
+    want = [step(l.clone().requires_grad_(), y.clone().requires_grad_(), d) for l, y, d in zip(logits, ys, douts)]
+    l, y, d = logits[0].clone().requires_grad_(), ys[0].clone().requires_grad_(), douts[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(l, y, d)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(l, y, d)
+    for _ in range(2):
+        for i in range(3):
+            with torch.no_grad():
+                l.copy_(logits[i])
+                y.copy_(ys[i])
+            d.copy_(douts[i])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+            step(logits[2].clone().requires_grad_(), ys[2].clone().requires_grad_(), douts[2])
+
+
+def test_large_numbers_of_rows_and_a_long_row(dev):
+    """Every row of a long batch, spread over many workgroups, and slots past 2^16 of one expert."""
+    from nerfhip import experts
+    T, E = 200003, 6
+    x = torch.randn(T, E, generator=torch.Generator().manual_seed(8)).half()
+    bias = torch.tensor([0.0, 0.5, -0.25, 0.125, 0.0, 0.3])
+    w, e = experts.route(x.to(dev), 2, score="sigmoid", bias=bias.to(dev))
+    want = ref_choice(x, 2, "sigmoid", bias, 1, 1, "max")
+    assert torch.equal(e.cpu().long(), want)
+    p = experts.plan(torch.zeros(T, 2, dtype=torch.int32, device=dev), E)
+    assert p.order.tolist() == list(range(2 * T)) and p.offsets.tolist() == [0] + [2 * T] * E

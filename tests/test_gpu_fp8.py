@@ -197,6 +197,33 @@ def test_expert_linear(dev, T, k, E, N, K, dt):
     assert torch.equal(experts.expert_linear(rows, f, p, bias=bias.to(dev), relu=True), y)
 
 
+@pytest.mark.parametrize("n", [24, 700])
+def test_rows_that_a_plan_leaves_out(dev, n):
+    """A plan made by hand: sorted rows whose slot is no row of x count as rows of zeros (bias alone), in the
+    skinny and the tiled form; sorted rows behind the last expert's become zeros."""
+    from nerfhip import experts
+    E, N, K = 2, 40, 200
+    _, f = make_weight(dev, E, N, K)
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, K, generator=g)
+    bias = torch.randn(E, N, generator=g)
+    order = torch.randperm(n, generator=g).int()
+    order[::3] = -1
+    order[1] = 2 ** 31 - 1
+    order[2] = n
+    off = torch.tensor([0, n // 2, n - 5], dtype=torch.int32)
+    p = experts.Plan(order.to(dev), torch.zeros(n, 1, dtype=torch.int32, device=dev), off.to(dev))
+    y = experts.expert_linear(x.to(dev), f, p, gather=True, bias=bias.to(dev)).cpu()
+    xq, wq = rows8(x), f.dequantize().cpu().double()
+    for e in range(E):
+        rows = torch.arange(int(off[e]), int(off[e + 1]))
+        src = order[rows].long()
+        live = (src >= 0) & (src < n)
+        assert bool((y[rows[~live]] == bias[e]).all())
+        check(y[rows[live]], xq[src[live]], wq[e], bias[e], False, torch.float32)
+    assert bool((y[n - 5:] == 0).all())
+
+
 def test_served_experts_end_to_end(dev):
     """Gate, plan, two 8-bit layers and the join, for a batch and for a single row (which takes the
     skinny form): row by row against the 64-bit form with the same roundings between the layers."""
