@@ -274,30 +274,58 @@ __device__ __forceinline__ bool find_tile(const LinearArgs& a, int tile, int& e,
   return false;
 }
 
-// This lane's columns' bias (zeros without).
+// This lane's columns' bias (zeros without) in a tile from column n0 on.
 template <class S>
-__device__ __forceinline__ void load_bias(const LinearArgs& a, int64_t e, int64_t n, float (&bias)[4 * S::TN]) {
+__device__ __forceinline__ void load_bias(const LinearArgs& a, const TileProduct<S>& p, int64_t e, int64_t n0,
+                                          float (&bias)[4 * S::TN]) {
 #pragma unroll
-  for (int c = 0; c < 4 * S::TN; ++c) bias[c] = a.bias && n + c < a.N ? a.bias[e * a.N + n + c] : 0.0f;
+  for (int c = 0; c < 4 * S::TN; ++c) {
+    const int64_t n = n0 + p.n(c / 8) + c % 8;
+    bias[c] = a.bias && n < a.N ? a.bias[e * a.N + n] : 0.0f;
+  }
 }
 
 // The tile's results: bias, ReLU, one rounding, rows below hi.
 template <class S, class T>
 __device__ __forceinline__ void store_tile(const LinearArgs& a, const TileProduct<S>& p, const float (&bias)[4 * S::TN],
                                            int64_t m0, int64_t hi, int64_t n0) {
-  const int64_t n = n0 + p.n();
   const bool vec = ((uintptr_t)a.out | (uintptr_t)(a.ldo * sizeof(T))) % 16 == 0;
+  auto value = [&](int i, int h, float (&v)[8]) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      v[c] = p.acc[i][2 * h + c / 4][c % 4] + bias[8 * h + c];
+      if (a.relu) v[c] = relu_of(v[c]);
+    }
+  };
+  // whole rows of the tile: no question but the row's (a branch around every store cost 76 us against 62 over
+  // 2^18 rows through 256 x 256)
+  if (vec && n0 + S::BN <= a.N) {
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i) {
+      const int64_t m = m0 + p.m(i);
+      T* row = (T*)a.out + m * a.ldo + n0;
+      if (m < hi) {
+#pragma unroll
+        for (int h = 0; h < S::TN / 2; ++h) {
+          float v[8];
+          value(i, h, v);
+          store_run(row + p.n(h), v, 8, true);
+        }
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < S::TM; ++i) {
     const int64_t m = m0 + p.m(i);
-    if (m < hi && n < a.N) {
-      float v[4 * S::TN];
 #pragma unroll
-      for (int c = 0; c < 4 * S::TN; ++c) {
-        v[c] = p.acc[i][c / 4][c % 4] + bias[c];
-        if (a.relu) v[c] = relu_of(v[c]);
+    for (int h = 0; h < S::TN / 2; ++h) {
+      const int64_t n = n0 + p.n(h);
+      if (m < hi && n < a.N) {
+        float v[8];
+        value(i, h, v);
+        store_run((T*)a.out + m * a.ldo + n, v, a.N - n, vec);
       }
-      store_run((T*)a.out + m * a.ldo + n, v, a.N - n, vec);
     }
   }
 }
@@ -391,7 +419,7 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
     tile_steps<S, kLoads>(a.KB, plan, load, chunk, scales);
   }
   float bias[4 * S::TN] = {};
-  if (!none) load_bias<S>(a, eb, n0 + p.n(), bias);
+  if (!none) load_bias<S>(a, p, eb, n0, bias);
   store_tile<S, T>(a, p, bias, m0, hi, n0);
 }
 
@@ -427,7 +455,7 @@ __global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int
   const int nb = (w % S::WC) * 16 * S::TN / 128;
 #pragma unroll
   for (int k = 0; k < KB; ++k) sn[k] = a.ws[(nb < a.NB ? nb : a.NB - 1) * KB + k];
-  load_bias<S>(a, 0, p.n(), bias);
+  load_bias<S>(a, p, 0, 0, bias);
   X x[IT][8];
   auto fetch = [&](int64_t tile) {
 #pragma unroll
@@ -459,7 +487,7 @@ __global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int
       int2 v;
       v.x = pack4(f[0], f[1], f[2], f[3]);
       v.y = pack4(f[4], f[5], f[6], f[7]);
-      *(int2*)(mine + kb * S::BM * 128 + r * 128 + (((l >> 1) ^ swz<S::TM>(r)) << 4) + (l & 1) * 8) = v;
+      *(int2*)(mine + kb * S::BM * 128 + r * 128 + (((l >> 1) ^ swz<S::R>(r)) << 4) + (l & 1) * 8) = v;
       if (l == 0) smine[kb * S::BM + r] = (unsigned char)sc;
     }
     const int64_t next = tile + gridDim.x;
@@ -748,7 +776,7 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   using SW = TileShape<Fp8Wide, 4, 4, 2, 2>;
   // 256 x 256 (128 x 128 for a wave, the whole register file) reads half as much LDS for each product,
   // but one workgroup on a CU has nobody to cover its start and end: for long rows and many tiles
-  // (8192 x 8192 x 8192: 534 us against 591; 32768 rows of 2048 over 32 experts: 269 against 243).
+  // (8192 x 8192 x 8192: 484 us against 632; 32768 rows of 2048 over 32 experts: 256 against 235).
   using SL = TileShape<Fp8, 8, 8, 2, 2>;
   const bool large = d->K >= 4096 && cdiv(d->M, 256) * cdiv(d->N, 256) >= 512;
   // 64 x 64 where the larger tiles would leave CUs without one.

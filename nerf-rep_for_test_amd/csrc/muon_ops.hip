@@ -313,8 +313,6 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
         p.chunk(stage, stage + S::BM * 128, kLoads, part);
       },
       [](int) {});
-  // this lane's rows m, columns n .. n + 4 TN
-  const int n = n0 + p.n();
   char* to = STEP == kStepA ? w.a : (STEP == kStepB ? w.b : w.xs);
   const char* add = STEP == kStepB ? w.a : w.xs;   // the term beside the product
   const int64_t lto = row_bytes(cols);
@@ -331,7 +329,7 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
     for (int h = 0; h < 4 * TN; h += 8) {
       HiLo v[8];
       float f[8];
-      const int nn = n + h;
+      const int nl = p.n(h / 8), nn = n0 + nl;
       f16x8 ah = {}, al = {};
       if (STEP != kStepA && m < rows && nn < cols) {
         const char* at = add + m * lto + (nn >> 5) * 128 + (nn & 31) * 2;
@@ -354,7 +352,7 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
         for (int e = 0; e < 8; ++e) f[e] *= 1.0f / g.s;
         if (tall) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tr[(p.n() + h + e) * PITCH + ml] = __float_as_uint(f[e]);
+          for (int e = 0; e < 8; ++e) tr[(nl + e) * PITCH + ml] = __float_as_uint(f[e]);
         } else if (m < rows) {
           finish<T>((T*)g.out + i * g.out_stride + (int64_t)m * g.n + nn, f, cols - nn, g.buf != nullptr, keep, rate);
         }
@@ -362,7 +360,7 @@ __global__ __launch_bounds__(S::NT) void muon_product_kernel(const Batch bt, int
         if (m < rows && nn < ((cols + 31) & ~31)) put8(to + m * lto, nn, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          tr[(p.n() + h + e) * PITCH + ml] =
+          tr[(nl + e) * PITCH + ml] =
               (unsigned)__builtin_bit_cast(unsigned short, v[e].hi) | (unsigned)__builtin_bit_cast(unsigned short, v[e].lo) << 16;
       }
     }

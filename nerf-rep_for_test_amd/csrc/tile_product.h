@@ -104,26 +104,32 @@ struct TileShape {
   using Mode = MODE;
   static constexpr int NS = NS_;
   static constexpr int TM = TM_, TN = TN_, WR = WR_, WC = WC_;
+  static constexpr int R = TM == 4 && TN == 4 && !std::is_same<MODE, Split>::value ? 4 : 2;   // see tile_row
   static constexpr int BM = 16 * TM * WR, BN = 16 * TN * WC, NT = 64 * WR * WC;
   static constexpr int kStage = (BM + BN) * 128;   // bytes of one stage
   static constexpr int LA = BM * 8 / NT, LB = BN * 8 / NT;   // 16-byte pieces per thread
+  static_assert(TM % 2 == 0 && TN % 2 == 0, "tiles in pairs");
   static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0, "whole pieces per thread");
 };
 
-// Tile t, index a (0..15) of a wave's 16 T rows <-> row (a / 4) 4 T + 4 t + a % 4: a lane's
-// results of all its tiles are then 4 T neighbours.
-template <int T>
+// Tile t, index a (0..15) of a wave's 16 T rows <-> row: the rows of R tiles are mixed so that a lane's
+// results of them are 4 R neighbours, (a / 4) 4 R + 4 (t % R) + a % 4, the next R tiles 16 R rows on.
+// R = 2: the 4 lanes of a row write 64 bytes of 16-bit results with each store; R = 4: each lane 32
+// neighbouring bytes with two. Measured both ways: 8 x 8 tiles of 8-bit products (8192 x 8192 x 8192) 534 us with
+// 2, 567 with 8; 4 x 4 tiles (2^18 rows through 256 x 256) 65 us with 2, 62 with 4; the FP16-split
+// ones 832 us with 2, 863 with 4 (32 matrices of 512 x 1024).
+template <int R>
 __device__ __forceinline__ constexpr int tile_row(int t, int a) {
-  return (a >> 2) * 4 * T + 4 * t + (a & 3);
+  return (t / R) * 16 * R + (a >> 2) * 4 * R + (t % R) * 4 + (a & 3);
 }
-template <int T>
+template <int R>
 __device__ __forceinline__ constexpr int swz(int r) {
-  return ((r / (4 * T)) & 3) * 2 + ((r >> 1) & 1);
+  return ((r / (4 * R)) & 3) * 2 + ((r >> 1) & 1);
 }
 
 template <class S>
 struct TileProduct {
-  static constexpr int TM = S::TM, TN = S::TN;
+  static constexpr int TM = S::TM, TN = S::TN, R = S::R;
   f32x4 acc[TM][TN];
   const char* a0;          // the tile's first rows
   const char* b0;
@@ -144,7 +150,7 @@ struct TileProduct {
     a0 = (const char*)uniform((int64_t)base);
 #pragma unroll
     for (int i = 0; i < S::LA; ++i) {
-      const int idx = i * S::NT + (int)threadIdx.x, r = idx >> 3, p = (idx & 7) ^ swz<TM>(r);
+      const int idx = i * S::NT + (int)threadIdx.x, r = idx >> 3, p = (idx & 7) ^ swz<R>(r);
       va[i] = row(r) * lda + p * 16;
     }
     set_n(B, ldb, n0, N);
@@ -165,7 +171,7 @@ struct TileProduct {
     const int bm = (int)(N - 1 - n0 < S::BN ? N - 1 - n0 : S::BN);
 #pragma unroll
     for (int i = 0; i < S::LB; ++i) {
-      const int idx = i * S::NT + t, r = idx >> 3, p = (idx & 7) ^ swz<TN>(r);
+      const int idx = i * S::NT + t, r = idx >> 3, p = (idx & 7) ^ swz<R>(r);
       vb[i] = (unsigned)(r < bm ? r : bm) * (unsigned)ldb + p * 16;
     }
   }
@@ -202,14 +208,14 @@ struct TileProduct {
   __device__ __forceinline__ void read(Frags& f, const char* sa, const char* sb, int d) const {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, a = lane & 15;
     if (d < TN) {
-      const int r = (w % S::WC) * 16 * TN + tile_row<TN>(d, a);
-      f.n[d][0] = *(const i32x4*)(sb + r * 128 + ((g ^ swz<TN>(r)) << 4));
-      f.n[d][1] = *(const i32x4*)(sb + r * 128 + (((g + 4) ^ swz<TN>(r)) << 4));
+      const int r = (w % S::WC) * 16 * TN + tile_row<R>(d, a);
+      f.n[d][0] = *(const i32x4*)(sb + r * 128 + ((g ^ swz<R>(r)) << 4));
+      f.n[d][1] = *(const i32x4*)(sb + r * 128 + (((g + 4) ^ swz<R>(r)) << 4));
     }
     if (d < TM) {
-      const int r = (w / S::WC) * 16 * TM + tile_row<TM>(d, a);
-      f.m[d][0] = *(const i32x4*)(sa + r * 128 + ((g ^ swz<TM>(r)) << 4));
-      f.m[d][1] = *(const i32x4*)(sa + r * 128 + (((g + 4) ^ swz<TM>(r)) << 4));
+      const int r = (w / S::WC) * 16 * TM + tile_row<R>(d, a);
+      f.m[d][0] = *(const i32x4*)(sa + r * 128 + ((g ^ swz<R>(r)) << 4));
+      f.m[d][1] = *(const i32x4*)(sa + r * 128 + (((g + 4) ^ swz<R>(r)) << 4));
     }
   }
 
@@ -289,15 +295,15 @@ struct TileProduct {
     }, parts, part);
   }
 
-  // This lane's result rows and columns within the workgroup's tile: tile i -> row m(i),
-  // columns n() .. n() + 4 TN (acc[i][j][r] is column n() + 4 j + r).
+  // This lane's results within the workgroup's tile: tile i's are of row m(i); columns n(h) .. n(h) + 8 are
+  // acc[i][2 h][0 .. 4], acc[i][2 h + 1][0 .. 4].
   __device__ __forceinline__ int m(int i) const {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    return (w / S::WC) * 16 * TM + tile_row<TM>(i, lane & 15);
+    return (w / S::WC) * 16 * TM + tile_row<R>(i, lane & 15);
   }
-  __device__ __forceinline__ int n() const {
+  __device__ __forceinline__ int n(int h) const {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    return (w % S::WC) * 16 * TN + (lane >> 4) * 4 * TN;
+    return (w % S::WC) * 16 * TN + (h / (R / 2)) * 16 * R + (lane >> 4) * 4 * R + h % (R / 2) * 8;
   }
 };
 
