@@ -79,7 +79,9 @@ class HipAdam(torch.optim.Adam):
         if g.get("amsgrad") or g.get("maximize") or g["weight_decay"] != 0:
             raise ValueError("HipAdam: amsgrad / maximize / weight decay are not supported")
         lr = g["lr"]
-        if not torch.is_tensor(lr):   # a float lr set by someone else: back on the device
+        if not torch.is_tensor(lr) or lr.device != self._count.device or lr.dtype != torch.float32:
+            # a float set by someone else, or a tensor of a state dict loaded to another device: the
+            # kernel reads one float32 of this device
             lr = g["lr"] = torch.tensor(float(lr), device=self._count.device)
         rows = []
         missing = [p for p in g["params"] if p.grad is None]
