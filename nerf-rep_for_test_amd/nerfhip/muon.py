@@ -175,6 +175,8 @@ class HipMuon(torch.optim.Optimizer):
     def step(self, closure=None):
         if closure is not None:
             raise ValueError("HipMuon.step takes no closure")
+        if len(self.param_groups) != (1 if self.adam is None else 2):
+            raise ValueError("HipMuon keeps its own two parameter groups: none can be added")
         g = self.param_groups[0]
         missing = [p for h in self.param_groups for p in h["params"] if p.grad is None]
         every = sum(len(h["params"]) for h in self.param_groups)
@@ -183,7 +185,8 @@ class HipMuon(torch.optim.Optimizer):
                 return None
             raise ValueError(f"HipMuon: {len(missing)} of {every} parameters have no gradient")
         lr = g["lr"]
-        if not torch.is_tensor(lr):   # a float lr set by someone else: back on the device
+        if not torch.is_tensor(lr) or lr.device != self._lr.device or lr.dtype != torch.float32:
+            # a float set by someone else, or a tensor of a state dict loaded to another device
             lr = g["lr"] = torch.tensor(float(lr), device=self._lr.device)
         buffers = []
         for p in g["params"]:

@@ -288,3 +288,35 @@ def test_calls_on_another_stream_and_in_a_graph(dev):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
             step(xs[2], lg[2])       # eager work between the replays
+
+
+def test_two_streams_at_once(dev):
+    """Products of every form on two streams, nothing waiting between: as one after the other."""
+    from nerfhip import experts, fp8
+    _, f1 = make_weight(dev, 300, 700, seed=1)
+    _, f2 = make_weight(dev, 256, 200, seed=2)
+    _, fe = make_weight(dev, 8, 96, 260, seed=3)
+    xs = [torch.randn(m, 700, device=dev) for m in (1, 20, 500, 1300)]
+    ys = [torch.randn(m, 200, device=dev).bfloat16() for m in (7, 40000, 33000, 600)]
+    zs = [torch.randn(m, 260, device=dev) for m in (5, 50, 400, 900)]
+    plans = [experts.plan(torch.randint(-1, 8, (z.shape[0], 3), device=dev, dtype=torch.int32), 8) for z in zs]
+
+    def first(i):
+        return fp8.linear(xs[i], f1), experts.expert_linear(zs[i], fe, plans[i], gather=True)
+
+    def second(i):
+        return (fp8.linear(ys[i], f2),)
+
+    want = [(*first(i), *second(i)) for i in range(4)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for i in range(4):
+        with torch.cuda.stream(s1):
+            a = first(i)
+        with torch.cuda.stream(s2):
+            b = second(i)
+        got.append((*a, *b))
+    torch.cuda.synchronize()
+    for u, v in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(u, v))

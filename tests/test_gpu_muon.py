@@ -230,6 +230,48 @@ def test_hip_muon_splits_the_parameters(dev):
         opt.step()
 
 
+def test_hip_muon_of_matrices_alone(dev):
+    """No other parameters; a learning rate on the host, then a float; a group that was added is refused."""
+    from nerfhip.muon import HipMuon
+    p0, g = torch.randn(40, 30, device=dev), torch.randn(40, 30, device=dev)
+    outs = []
+    for lr in (None, torch.tensor(2e-3), torch.tensor(2e-3, dtype=torch.float64), 2e-3):
+        p = p0.clone().requires_grad_()
+        opt = HipMuon([p], lr=2e-3, weight_decay=0.1)
+        if lr is not None:
+            opt.param_groups[0]["lr"] = lr
+        for _ in range(2):
+            p.grad = g.clone()
+            opt.step()
+        outs.append(p.detach())
+    assert all(torch.equal(outs[0], v) for v in outs[1:]) and not torch.equal(outs[0], p0)
+    opt.zero_grad()
+    assert opt.step() is None
+    opt.add_param_group({"params": [torch.zeros(16, 16, device=dev, requires_grad=True)]})
+    with pytest.raises(ValueError, match="groups"):
+        opt.step()
+
+
+def test_two_streams_at_once(dev):
+    """Steps of two optimisers' matrices and an orthogonalisation on two streams, nothing waiting between: as one
+    after the other."""
+    from nerfhip import muon
+    ga = [torch.randn(2, 300, 500, device=dev) for _ in range(6)]
+    gb = [torch.randn(5, 100, 40, device=dev) for _ in range(6)]
+    want = [(muon.orthogonalize(a), muon.orthogonalize(b)) for a, b in zip(ga, gb)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for a, b in zip(ga, gb):
+        with torch.cuda.stream(s1):
+            x = muon.orthogonalize(a)
+        with torch.cuda.stream(s2):
+            y = muon.orthogonalize(b)
+        got.append((x, y))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) and torch.equal(b, d) for (a, b), (c, d) in zip(got, want))
+
+
 @pytest.mark.parametrize("n_importance", [128, 0])
 def test_trainer_steps_with_muon(dev, n_importance):
     """NerfTrainer(adam="muon"): graph steps (two eager, the capture, replays) equal eager ones bit for bit, the
@@ -248,7 +290,7 @@ def test_trainer_steps_with_muon(dev, n_importance):
         torch.manual_seed(5)
         tr = NerfTrainer(dev, params_of(z), N_importance=n_importance, graph=graph, adam="muon", lr=1e-4)
         first = {k: v.clone() for k, v in tr.state().items()}
-        losses = [float(tr.step(ro, rd, gt)["loss"]) for _ in range(6)]
+        losses = [tr.step(ro, rd, gt)["loss"].item() for _ in range(6)]
         runs.append((losses, {k: v.clone() for k, v in tr.state().items()}, tr))
     assert runs[0][0] == runs[1][0]
     for k, v in runs[0][1].items():
