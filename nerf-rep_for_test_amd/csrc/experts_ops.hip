@@ -46,9 +46,11 @@ __device__ __forceinline__ unsigned reduce32(unsigned v, OP op) {
   v = op(v, dpp<0x4E>(v));    // lane ^ 2
   v = op(v, dpp<0x141>(v));   // the other four of 8
   v = op(v, dpp<0x140>(v));   // the other eight of 16
-  if constexpr (L == 64) {
-    v = op(v, (unsigned)__shfl_xor((int)v, 16));
-    v = op(v, (unsigned)__shfl_xor((int)v, 32));
+  if constexpr (L == 64) {   // the lanes 16 and 32 away, without LDS: a value swapped with itself
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(b[0], b[1]);
   }
   return v;
 }
@@ -68,12 +70,6 @@ template <int L>
 __device__ __forceinline__ unsigned row_or(unsigned v) {
   return reduce32<L>(v, [](unsigned a, unsigned b) { return a | b; });
 }
-template <int L>
-__device__ __forceinline__ double row_sum(double v) {
-  for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d);
-  return v;
-}
-
 // LDS written by a row's lanes (all of one wave) may be read by them.
 __device__ __forceinline__ void row_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
@@ -97,17 +93,31 @@ template <int CTRL>
 __device__ __forceinline__ double dpp64(double v) {
   return __hiloint2double((int)dpp<CTRL>((unsigned)__double2hiint(v)), (int)dpp<CTRL>((unsigned)__double2loint(v)));
 }
-template <int L>
-__device__ __forceinline__ double row_max(double v) {
-  v = fmax(v, dpp64<0xB1>(v));
-  v = fmax(v, dpp64<0x4E>(v));
-  v = fmax(v, dpp64<0x141>(v));
-  v = fmax(v, dpp64<0x140>(v));
+template <int L, class OP>
+__device__ __forceinline__ double reduce64(double v, OP op) {
+  v = op(v, dpp64<0xB1>(v));
+  v = op(v, dpp64<0x4E>(v));
+  v = op(v, dpp64<0x141>(v));
+  v = op(v, dpp64<0x140>(v));
   if constexpr (L == 64) {
-    v = fmax(v, __shfl_xor(v, 16));
-    v = fmax(v, __shfl_xor(v, 32));
+    const unsigned lo = (unsigned)__double2loint(v), hi = (unsigned)__double2hiint(v);
+    const auto l16 = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto h16 = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    v = op(__hiloint2double((int)h16[0], (int)l16[0]), __hiloint2double((int)h16[1], (int)l16[1]));
+    const unsigned lo2 = (unsigned)__double2loint(v), hi2 = (unsigned)__double2hiint(v);
+    const auto l32 = __builtin_amdgcn_permlane32_swap(lo2, lo2, false, false);
+    const auto h32 = __builtin_amdgcn_permlane32_swap(hi2, hi2, false, false);
+    v = op(__hiloint2double((int)h32[0], (int)l32[0]), __hiloint2double((int)h32[1], (int)l32[1]));
   }
   return v;
+}
+template <int L>
+__device__ __forceinline__ double row_max(double v) {
+  return reduce64<L>(v, [](double a, double b) { return fmax(a, b); });
+}
+template <int L>
+__device__ __forceinline__ double row_sum(double v) {
+  return reduce64<L>(v, [](double a, double b) { return a + b; });
 }
 // A sorting network (merge exchange) for a power of two of values, the largest first.
 template <int N>
@@ -130,14 +140,9 @@ __device__ __forceinline__ void sort_down(double (&v)[N]) {
 // (key, index) with the higher key, or at equal keys the lower index, over the lanes of a row.
 template <int L>
 __device__ __forceinline__ void row_best(double& key, int& idx) {
-  for (int d = 1; d < L; d *= 2) {
-    const double k2 = __shfl_xor(key, d);
-    const int i2 = __shfl_xor(idx, d);
-    if (k2 > key || (k2 == key && i2 < idx)) {
-      key = k2;
-      idx = i2;
-    }
-  }
+  const double m = row_max<L>(key);
+  idx = (int)reduce32<L>(key == m ? (unsigned)idx : ~0u, [](unsigned a, unsigned b) { return a < b ? a : b; });
+  key = m;
 }
 
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
@@ -180,15 +185,19 @@ __device__ __forceinline__ F ranked(F key) {
   return key > lowest<F>() ? key : lowest<F>();
 }
 
+// An expert's group: a shift where groups have a power of two of experts (bits >= 0).
+__device__ __forceinline__ int per_bits(int per) { return per & (per - 1) ? -1 : 31 - __builtin_clz(per); }
+__device__ __forceinline__ int group_of(int e, int per, int bits) { return bits >= 0 ? e >> bits : e / per; }
+
 // The groups that stay (bits) by the highest or two highest of their keys; `doubt`: whether the last
 // one kept and the first one dropped are nearer than `tol`.
 template <class F, int L, int V>
 __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, const F (&key)[V], F* ks, int lane, F tol,
                                                           bool& doubt) {
-  const int per = a.E / a.groups;
+  const int per = a.E / a.groups, bits = per_bits(per);
   F* gs = ks + a.E + a.groups;
   auto score = [&](F b1, F b2) { return a.group_top2 && per > 1 ? (b2 > lowest<F>() ? b1 + b2 : lowest<F>()) : b1; };
-  if (sizeof(F) == 4 && per >= 4 && per <= 64 && (per & (per - 1)) == 0) {
+  if (sizeof(F) == 4 && per >= 4 && per <= 64 && bits >= 0) {
     // a group is whole lanes' runs of 4: the two highest by DPP
 #pragma unroll
     for (int v = 0; v < V; v += 4) {
@@ -204,14 +213,14 @@ __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, co
       if (per > 16) add(dpp_f<0x141>(b1), dpp_f<0x141>(b2));
       if (per > 32) add(dpp_f<0x140>(b1), dpp_f<0x140>(b2));
       const int e = expert_of<L>(lane, v);
-      if (e < a.E && e % per == 0) gs[e / per] = score(b1, b2);
+      if (e < a.E && (e & (per - 1)) == 0) gs[e >> bits] = score(b1, b2);
     }
   } else {
     // through LDS, lane j takes group j
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int e = expert_of<L>(lane, v);
-      if (e < a.E) ks[e + e / per] = key[v];   // (a word between groups: they lie in different banks)
+      if (e < a.E) ks[e + group_of(e, per, bits)] = key[v];   // (a word between groups: they lie in different banks)
     }
     row_fence();
     for (int j = lane; j < a.groups; j += L) {
@@ -232,6 +241,7 @@ __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, co
   for (int j = lane; j < a.groups; j += L) {
     const F mine = gs[j];
     int better = 0;
+#pragma unroll 8
     for (int i = 0; i < a.groups; ++i) better += gs[i] > mine || (gs[i] == mine && i < j);
     if (better < a.top_groups) {
       lo |= j < 32 ? 1u << j : 0u;
@@ -263,7 +273,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
   float key[V];
   float tol = 0.0f;   // twice two keys' errors, apart from their last rounding
   const bool scored = a.bias != nullptr || (a.groups > 1 && a.group_top2);
-  const int per = a.E / a.groups;
+  const int per = a.E / a.groups, bits = per_bits(per);
   if (scored) {
     scores<float, L, V>(a, x, top, lane, key);
     // sigmoid: 3 steps of a score (at most 1). Softmax: 1.2e-6 of one (the sum of 1024 terms: 20 steps),
@@ -305,7 +315,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
       const int e = expert_of<L>(lane, v);
       if (e < a.E) {
         if (!a.bias) key[v] = ranked(x[v]);   // the order of the logits
-        if (!((keep >> (e / per)) & 1)) key[v] = -__builtin_inff();
+        if (!((keep >> group_of(e, per, bits)) & 1)) key[v] = -__builtin_inff();
       }
     }
   }
