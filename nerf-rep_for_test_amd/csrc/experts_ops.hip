@@ -70,9 +70,10 @@ template <int L>
 __device__ __forceinline__ unsigned row_or(unsigned v) {
   return reduce32<L>(v, [](unsigned a, unsigned b) { return a | b; });
 }
-// LDS written by a row's lanes (all of one wave) may be read by them.
+// LDS written by a row's lanes (all of one wave) may be read by them: a wave's LDS accesses are done in
+// their order, so only the compiler has to keep it (a workgroup's fence would wait for stores to memory).
 __device__ __forceinline__ void row_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
 
@@ -589,7 +590,8 @@ __global__ __launch_bounds__(256) void route_backward_kernel(const RouteBwdArgs 
 // A stable counting sort of the n slots by expert. A wave counts, and later places, a run of
 // neighbouring slots, 64 at a time in order: lanes with the same expert are found by ballots over
 // the bits of its number, so the places follow from counts alone (no atomics that decide an order).
-// Bound by the latency of its launches: 131072 slots in 4 + 2 + 5 us, up to 4096 in one launch (4 us).
+// Bound by the latency of its launches: 131072 slots in 4 + 2 + 5 us. Up to 8192 slots one workgroup does it
+// all (8168 slots of 256 experts: 14 us a call, three launches 19; 16384: 25 and 19).
 __device__ __forceinline__ unsigned long long same_expert(int e, bool live, int bits) {
   unsigned long long peers = __ballot(live);
   for (int b = 0; b < bits; ++b) {
@@ -601,36 +603,45 @@ __device__ __forceinline__ unsigned long long same_expert(int e, bool live, int 
 }
 
 constexpr int kPlanSegs = 1024;   // runs of slots (one wave each) of a large plan
-constexpr int kPlanSmall = 4096;  // up to here one workgroup does everything (LDS: 18 words an expert)
+constexpr int kPlanSmall = 8192;  // up to here one workgroup does everything (LDS: 18 words an expert)
 bool plan_is_small(int64_t n, int E) { return n <= kPlanSmall && E <= 512; }
 
 __device__ __forceinline__ void plan_count(const int* experts, int64_t lo, int64_t hi, int E, int* cnt, int lane, int bits) {
-  for (int64_t i = lo; i < hi; i += 64) {
-    const int e = i + lane < hi ? experts[i + lane] : -1;
-    const bool live = e >= 0 && e < E;
-    const unsigned long long peers = same_expert(e, live, bits);
-    if (live && __builtin_ctzll(peers) == lane) cnt[e] += __builtin_popcountll(peers);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
+  for (int64_t i0 = lo; i0 < hi; i0 += 256) {
+    int ex[4];   // (4 times 64 slots on their way at once)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) ex[u] = i0 + u * 64 + lane < hi ? experts[i0 + u * 64 + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = ex[u];
+      const bool live = e >= 0 && e < E;
+      const unsigned long long peers = same_expert(e, live, bits);
+      if (live && __builtin_ctzll(peers) == lane) cnt[e] += __builtin_popcountll(peers);
+      row_fence();
+    }
   }
 }
 
 __device__ __forceinline__ void plan_place(const int* experts, int64_t lo, int64_t hi, int E, int* at, int lane, int bits,
                                            int* order, int* position) {
-  for (int64_t i = lo; i < hi; i += 64) {
-    const bool in = i + lane < hi;
-    const int e = in ? experts[i + lane] : -1;
-    const bool live = e >= 0 && e < E;
-    const unsigned long long peers = same_expert(e, live, bits);
-    int p = -1;
-    if (live) p = at[e] + __builtin_popcountll(peers & ((1ull << lane) - 1));
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    if (live && __builtin_ctzll(peers) == lane) at[e] += __builtin_popcountll(peers);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-    __builtin_amdgcn_wave_barrier();
-    if (in) position[i + lane] = p;
-    if (live) order[p] = (int)(i + lane);
+  for (int64_t i0 = lo; i0 < hi; i0 += 256) {
+    int ex[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) ex[u] = i0 + u * 64 + lane < hi ? experts[i0 + u * 64 + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = i0 + u * 64 + lane;
+      const int e = ex[u];
+      const bool live = e >= 0 && e < E;
+      const unsigned long long peers = same_expert(e, live, bits);
+      int p = -1;
+      if (live) p = at[e] + __builtin_popcountll(peers & ((1ull << lane) - 1));
+      row_fence();
+      if (live && __builtin_ctzll(peers) == lane) at[e] += __builtin_popcountll(peers);
+      row_fence();
+      if (i < hi) position[i] = p;
+      if (live) order[p] = (int)i;
+    }
   }
 }
 

@@ -234,7 +234,8 @@ def test_no_rows(dev):
 # ---------------------------------------------------------------- the plan
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 6, 64), (7, 3, 5), (1024, 4, 512), (1025, 4, 512), (4096, 1, 1000),
-                                   (2048, 2, 1024), (3, 32, 1024), (5000, 2, 16), (70001, 3, 100), (65536, 8, 256)])
+                                   (2048, 2, 1024), (3, 32, 1024), (5000, 2, 16),
+                                   (2048, 4, 100), (2731, 3, 200), (8191, 1, 513), (70001, 3, 100), (65536, 8, 256)])
 @pytest.mark.parametrize("holes", [False, True])
 def test_plan_is_the_stable_sort(dev, T, k, E, holes):
     from nerfhip import experts
