@@ -613,6 +613,7 @@ __device__ __forceinline__ void plan_count(const int* experts, int64_t lo, int64
     for (int u = 0; u < 4; ++u) ex[u] = i0 + u * 64 + lane < hi ? experts[i0 + u * 64 + lane] : -1;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      if (i0 + u * 64 >= hi) break;
       const int e = ex[u];
       const bool live = e >= 0 && e < E;
       const unsigned long long peers = same_expert(e, live, bits);
@@ -630,6 +631,7 @@ __device__ __forceinline__ void plan_place(const int* experts, int64_t lo, int64
     for (int u = 0; u < 4; ++u) ex[u] = i0 + u * 64 + lane < hi ? experts[i0 + u * 64 + lane] : -1;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      if (i0 + u * 64 >= hi) break;
       const int64_t i = i0 + u * 64 + lane;
       const int e = ex[u];
       const bool live = e >= 0 && e < E;
@@ -916,10 +918,11 @@ void go_route(const RouteArgs& a, const float* dw, void* dlogits, hipStream_t st
 
 template <class T, bool VEC>
 void go_route_e(const RouteArgs& a, const float* dw, void* dl, hipStream_t st) {
-  // 16 lanes for a row waste least (E = 256, k = 8, T = 65536: 32 us against 59 with 64 lanes), but with
-  // many experts and few rows the time is one row's, which more lanes shorten (T = 1021, sigmoid, bias and
-  // groups: 12.8 us against 18.9; at T = 4096 15.8 against 19.1, at 16384 34 against 30)
-  if (a.E > 128 && a.E <= 256 && a.T <= 4096) go_route<64, 4, T, VEC>(a, dw, dl, st);
+  // 16 lanes for a row waste least (E = 256, k = 8: T = 65536 in 32 us against 59 with 64 lanes, 16384 in 10
+  // against 21), but with many experts and few rows the time is one row's, which more lanes shorten (T = 1021:
+  // 5.8 against 5.0 us; sigmoid, bias and groups 11.3 against 7.4, at T = 4096 16.1 against 13.1, at 8192 16.9
+  // against 19.5; without them 5.9 against 8.0 at 4096)
+  if (a.E > 128 && a.E <= 256 && a.T <= (a.bias || a.groups > 1 ? 4096 : 2048)) go_route<64, 4, T, VEC>(a, dw, dl, st);
   else if (a.E <= 64) go_route<16, 4, T, VEC>(a, dw, dl, st);
   else if (a.E <= 128) go_route<16, 8, T, VEC>(a, dw, dl, st);
   else if (a.E <= 256) go_route<16, 16, T, VEC>(a, dw, dl, st);
