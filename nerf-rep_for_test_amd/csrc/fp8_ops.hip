@@ -269,9 +269,8 @@ __device__ __forceinline__ bool find_tile(const LinearArgs& a, int tile, int& e,
       const int at = __builtin_ctzll(met);
       e = base + at;
       const int first = before + __shfl(sum - n, at);
-      expert_rows(a, e, l, h);
-      m0 = l + (int64_t)(tile - first) * BM;
-      hi = h;
+      m0 = __shfl((int)l, at) + (int64_t)(tile - first) * BM;   // (rows are below 2^31)
+      hi = __shfl((int)h, at);
       return true;
     }
     before += __shfl(sum, 63);
