@@ -120,10 +120,13 @@ def launch(x, weight, M, order, slots, offsets, bias, relu, out_dtype, who):
 
 def linear(x, weight, bias=None, relu=False, out_dtype=None):
     """y [.., N] = x [.., K] W^T (+ bias [N] float32, ReLU) with the activations rounded to
-    8-bit blocks of 128; sums in float32, y in ``out_dtype`` (default: x's type). A block with a
-    value that is not finite makes its row's outputs NaN."""
+    8-bit blocks of 128; sums in float32, y in ``out_dtype`` (default: x's type). float32 results have
+    exact products, 16-bit ones the 8-bit matrix instruction's (1e-5 of a result's norm, below their
+    rounding). A block with a value that is not finite makes its row's outputs NaN. K up to 2^23."""
     if not isinstance(weight, Fp8Weight) or weight.q.dim() != 2:
         raise ValueError("linear: weight must be an Fp8Weight of one matrix")
+    if weight.k > 1 << 23:
+        raise ValueError("linear: K up to 2^23")
     if x.dim() < 1 or x.shape[-1] != weight.k:
         raise ValueError(f"linear: activations must be [.., {weight.k}]")
     flat = x.reshape(-1, x.shape[-1])
