@@ -215,6 +215,13 @@ def enqueue(name: str, t, *args) -> None:
         check(rc, name)
 
 
+def written(*tensors) -> None:
+    """Raise the version counters of tensors that a kernel wrote in place, as torch's own in-place operations do:
+    the Renderer repacks its weights by them, and autograd refuses a backward pass over changed tensors."""
+    import torch
+    torch.autograd.graph.increment_version(tensors)
+
+
 def require_gpu(t) -> None:
     if not t.is_cuda:
         raise NerfHipError("nerfhip ops need tensors on a ROCm GPU (got %s); there is no CPU "

@@ -83,7 +83,7 @@ class HipAdam(torch.optim.Adam):
             # a float set by someone else, or a tensor of a state dict loaded to another device: the
             # kernel reads one float32 of this device
             lr = g["lr"] = torch.tensor(float(lr), device=self._count.device)
-        rows = []
+        rows, changed = [], [self._count]
         missing = [p for p in g["params"] if p.grad is None]
         if missing and len(missing) != len(g["params"]):
             raise ValueError(f"HipAdam: {len(missing)} of {len(g['params'])} parameters have no "
@@ -96,6 +96,7 @@ class HipAdam(torch.optim.Adam):
             for t in (p, gr, m, v):
                 if t.dtype != torch.float32 or not t.is_contiguous():
                     raise ValueError("HipAdam needs contiguous float32 tensors")
+            changed += (p, m, v) if self.clip < 0 else (p, m, v, gr)   # (clipping is in place)
             rows.append((p.data_ptr(), gr.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()))
         if not rows:
             return None
@@ -107,4 +108,5 @@ class HipAdam(torch.optim.Adam):
         call("nerf_adam_step", ctypes.addressof(self._arr), len(rows), lr.data_ptr(),
              self._count.data_ptr(), None, float(b1), float(b2),
              float(g["eps"]), self.clip, _lib.stream_of(self._count.device))
+        _lib.written(*changed)
         return None

@@ -118,6 +118,7 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     o = _Options(0, 1, int(bool(nesterov)), steps, 0.0 if dev_lr else float(lr), float(momentum), float(weight_decay),
                  float(eps), -1.0 if clip is None else float(clip), ptr(lr) if dev_lr else None)
     _run(groups, o, params[0])
+    _lib.written(*params, *momenta)
 
 
 def is_hidden_matrix(p):

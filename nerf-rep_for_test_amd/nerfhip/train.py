@@ -431,6 +431,7 @@ class NerfTrainer:
         if pairs:
             torch._foreach_copy_([d for d, _ in pairs], [s for _, s in pairs])
         graph.replay()
+        _lib.written(*self.trained_parameters())   # (the replay's kernels, not torch, wrote them)
         return out
 
     def _step_eager(self, rays_o, rays_d, target, t_rand=None, u=None, group=None):
