@@ -190,14 +190,22 @@ __device__ __forceinline__ F ranked(F key) {
 __device__ __forceinline__ int per_bits(int per) { return per & (per - 1) ? -1 : 31 - __builtin_clz(per); }
 __device__ __forceinline__ int group_of(int e, int per, int bits) { return bits >= 0 ? e >> bits : e / per; }
 
-// The groups that stay (bits) by the highest or two highest of their keys; `doubt`: whether the last
-// one kept and the first one dropped are nearer than `tol`.
+// The groups that stay (bits) by the highest or two highest of their keys; `doubt`: whether a dropped one may
+// lie above a kept one when each group is off by its scores' errors (`tol` for two groups together) and its keys'
+// roundings, which follow the keys' size and not their sum's (keys of a group may cancel): 2^-24 of
+// each key and of the sum, taken twice. Any dropped group may be the one, not the next alone.
 template <class F, int L, int V>
 __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, const F (&key)[V], F* ks, int lane, F tol,
                                                           bool& doubt) {
   const int per = a.E / a.groups, bits = per_bits(per);
   F* gs = ks + a.E + a.groups;
+  F* size = gs + a.groups;   // 32 bits: a group's |keys|, 0 for a score of the lowest
   auto score = [&](F b1, F b2) { return a.group_top2 && per > 1 ? (b2 > lowest<F>() ? b1 + b2 : lowest<F>()) : b1; };
+  auto put = [&](int j, F b1, F b2) {
+    const F s = score(b1, b2);
+    gs[j] = s;
+    if (sizeof(F) == 4) size[j] = s > lowest<F>() ? fabsf((float)b1) + (a.group_top2 && per > 1 ? fabsf((float)b2) : 0.0f) : 0.0f;
+  };
   if (sizeof(F) == 4 && per >= 4 && per <= 64 && bits >= 0) {
     // a group is whole lanes' runs of 4: the two highest by DPP
 #pragma unroll
@@ -214,7 +222,7 @@ __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, co
       if (per > 16) add(dpp_f<0x141>(b1), dpp_f<0x141>(b2));
       if (per > 32) add(dpp_f<0x140>(b1), dpp_f<0x140>(b2));
       const int e = expert_of<L>(lane, v);
-      if (e < a.E && (e & (per - 1)) == 0) gs[e >> bits] = score(b1, b2);
+      if (e < a.E && (e & (per - 1)) == 0) put(e >> bits, b1, b2);
     }
   } else {
     // through LDS, lane j takes group j
@@ -232,31 +240,31 @@ __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, co
         b2 = v > b1 ? b1 : (v > b2 ? v : b2);
         b1 = v > b1 ? v : b1;
       }
-      gs[j] = score(b1, b2);
+      put(j, b1, b2);
     }
   }
   row_fence();
   // a lane ranks its own groups; all of the row's lanes join their bits
   unsigned lo = 0, hi = 0;
-  F last = __builtin_inff(), first = -(F)__builtin_inff();   // lowest kept, highest dropped
+  F last = __builtin_inff(), first = -(F)__builtin_inff();   // lowest kept, highest dropped, by their errors
   for (int j = lane; j < a.groups; j += L) {
-    const F mine = gs[j];
+    const F mine = gs[j], err = sizeof(F) == 4 ? (F)2.4e-7f * size[j] : (F)0;
     int better = 0;
 #pragma unroll 8
     for (int i = 0; i < a.groups; ++i) better += gs[i] > mine || (gs[i] == mine && i < j);
     if (better < a.top_groups) {
       lo |= j < 32 ? 1u << j : 0u;
       hi |= j < 32 ? 0u : 1u << (j - 32);
-      last = mine < last ? mine : last;
+      last = mine - err < last ? mine - err : last;
     } else {
-      first = mine > first ? mine : first;
+      first = mine + err > first ? mine + err : first;
     }
   }
   const unsigned long long keep = (unsigned long long)row_or<L>(hi) << 32 | row_or<L>(lo);
   if (sizeof(F) == 4) {
     last = -row_max<L>((float)-last);
     first = row_max<L>((float)first);
-    doubt = a.top_groups < a.groups && first > lowest<F>() && last - first < tol + (F)4.8e-7 * (last < 0 ? -last : last);
+    doubt = a.top_groups < a.groups && first > lowest<F>() && last - first < tol;
   }
   return keep;
 }
