@@ -612,9 +612,9 @@ enum { NERF_F32 = 0, NERF_BF16 = 1, NERF_F16 = 2 };   /* element types */
  *   order is that of the logits). groups > 1: E / groups neighbours are a
  *   group; only the top_groups groups with the highest score (their highest
  *   key, or with group_top2 the sum of their two highest, from s + bias) stay.
- *   The k highest keys are chosen, as in exact arithmetic, ties to the lowest
- *   index; weights = scale * s, with renorm divided by the sum of the chosen s.
- *   NaN keys count as the lowest; a row that holds a NaN logit (or +inf under
+ *   The k highest keys are chosen, in the order of 64-bit keys, ties to the
+ *   lowest index; weights = scale * s, with renorm divided by the sum of the
+ *   chosen s. NaN and -inf keys are the lowest, below every number; a row that holds a NaN logit (or +inf under
  *   softmax) gets NaN weights, one whose (chosen) logits are all -inf zeros.
  *   E <= 1024, k <= 32, groups <= 64.
  * nerf_route_backward: d logits [T][E] (contiguous, the logits' type) from

@@ -148,10 +148,12 @@ __device__ __forceinline__ void row_best(double& key, int& idx) {
 
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
+// The least key, that of NaN and -inf: below every number that 32 bits hold, -3.4e38 (a mask of the type's
+// lowest value) too.
 template <class F>
 __device__ __forceinline__ F lowest();
 template <>
-__device__ __forceinline__ float lowest<float>() { return -3.402823466e+38f; }
+__device__ __forceinline__ float lowest<float>() { return -__builtin_inff(); }
 template <>
 __device__ __forceinline__ double lowest<double>() { return -1.7976931348623157e+308; }
 
@@ -180,7 +182,6 @@ __device__ __forceinline__ void scores(const RouteArgs& a, const float (&x)[V], 
   }
 }
 
-// NaN and -inf as the lowest number: in order before what is out of reach (-inf).
 template <class F>
 __device__ __forceinline__ F ranked(F key) {
   return key > lowest<F>() ? key : lowest<F>();
@@ -264,14 +265,15 @@ __device__ __forceinline__ unsigned long long keep_groups(const RouteArgs& a, co
   if (sizeof(F) == 4) {
     last = -row_max<L>((float)-last);
     first = row_max<L>((float)first);
-    doubt = a.top_groups < a.groups && first > lowest<F>() && last - first < tol;
+    // (not a number: both beyond 32 bits' range, or both the lowest)
+    doubt = a.top_groups < a.groups && !(last - first >= tol);
   }
   return keep;
 }
 
 // Chooses a row's k experts (into chosen[] in LDS, which its lanes read after a row_fence).
 //
-// The order is that of exact arithmetic. Without a bias the keys are the logits themselves; with
+// The order is that of 64-bit keys. Without a bias the keys are the logits themselves; with
 // one they are computed in 32 bits, and where two neighbours in the order (or the last group kept
 // and the first one dropped) are nearer than the keys' error and not made of equal inputs, in
 // 64 bits again: then only for the experts that can be among the first k (scores of a softmax: for
@@ -280,6 +282,7 @@ template <int L, int V, class T>
 __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const float (&x)[V], float top, double* lds, int* chosen,
                        int lane) {
   float key[V];
+  unsigned out = 0;       // bit v: out of reach (behind the last expert, or in a group that was dropped)
   float tol = 0.0f;   // twice two keys' errors, apart from their last rounding
   const bool scored = a.bias != nullptr || (a.groups > 1 && a.group_top2);
   const int per = a.E / a.groups, bits = per_bits(per);
@@ -297,11 +300,15 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int e = expert_of<L>(lane, v);
-      key[v] = e < a.E ? ranked(a.bias ? key[v] + a.bias[e] : key[v]) : -__builtin_inff();
+      key[v] = e < a.E ? ranked(a.bias ? key[v] + a.bias[e] : key[v]) : lowest<float>();
+      out |= e < a.E ? 0u : 1u << v;
     }
   } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = expert_of<L>(lane, v) < a.E ? ranked(x[v]) : -__builtin_inff();
+    for (int v = 0; v < V; ++v) {
+      key[v] = ranked(x[v]);
+      out |= expert_of<L>(lane, v) < a.E ? 0u : 1u << v;
+    }
   }
   unsigned long long keep = ~0ull;
   if (a.groups > 1) {
@@ -324,7 +331,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
       const int e = expert_of<L>(lane, v);
       if (e < a.E) {
         if (!a.bias) key[v] = ranked(x[v]);   // the order of the logits
-        if (!((keep >> group_of(e, per, bits)) & 1)) key[v] = -__builtin_inff();
+        if (!((keep >> group_of(e, per, bits)) & 1)) out |= 1u << v;
       }
     }
   }
@@ -332,9 +339,9 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
   float before = __builtin_inff();
   int ib = 0;
   const int rounds = a.bias && a.k < a.E ? a.k + 1 : a.k;   // one more: the first one left out
-  double order[V];   // a lane's keys, highest first
+  double order[V];   // a lane's keys, highest first; 0 (in key_of: NaN) behind them
 #pragma unroll
-  for (int v = 0; v < V; ++v) order[v] = pack_key(key[v], expert_of<L>(lane, v));
+  for (int v = 0; v < V; ++v) order[v] = out >> v & 1 ? 0.0 : pack_key(key[v], expert_of<L>(lane, v));
   sort_down<V>(order);
   auto take = [&](auto depth) {   // (a lane gives at most `rounds` of its keys)
     constexpr int D = decltype(depth)::value;
@@ -359,19 +366,19 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
   else take(std::integral_constant<int, V>());
   if (!doubt) return;
   // 64 bits, for the experts that may be among the first k: not below the k-th by more than the error
-  const float least = fmaxf(before - tol - 2.4e-7f * fabsf(before), lowest<float>());
+  const float least = fmaxf(before - tol - 2.4e-7f * fabsf(before), lowest<float>());   // (inf - inf: all of them)
   double k64[V];
   if (a.sigmoid) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       k64[v] = -(double)__builtin_inff();
-      if (key[v] >= least) k64[v] = ranked(1.0 / (1.0 + exp(-(double)x[v])) + (double)a.bias[expert_of<L>(lane, v)]);
+      if (key[v] >= least && !(out >> v & 1)) k64[v] = ranked(1.0 / (1.0 + exp(-(double)x[v])) + (double)a.bias[expert_of<L>(lane, v)]);
     }
   } else {
     scores<double, L, V>(a, x, top, lane, k64);
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      k64[v] = key[v] >= least ? ranked(k64[v] + (double)a.bias[expert_of<L>(lane, v)]) : -(double)__builtin_inff();
+      k64[v] = key[v] >= least && !(out >> v & 1) ? ranked(k64[v] + (double)a.bias[expert_of<L>(lane, v)]) : -(double)__builtin_inff();
   }
   row_fence();
   for (int j = 0; j < a.k; ++j) {

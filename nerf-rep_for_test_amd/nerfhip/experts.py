@@ -71,11 +71,11 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_s
     """(weights float32 [T, k], experts int32 [T, k]) of logits [T, E] (float32, bfloat16, float16).
 
     s = softmax or sigmoid (``score``) of a row; the k experts with the highest s + ``bias`` ([E] float32; it
-    only chooses, and has no gradient) in falling order, ties to the lowest index, as in exact arithmetic.
+    only chooses, and has no gradient) in falling order of the 64-bit keys, ties to the lowest index.
     ``groups`` > 1: only experts of the ``top_groups`` groups of E / groups neighbours with the highest
     ``group_score`` ("max": their highest s + bias, "top2": the sum of their two highest).
-    weights = ``scale`` * s, with ``renormalise`` divided by the sum of the row's chosen s. A NaN counts as
-    the lowest; a row that holds one (or +inf under softmax) has NaN weights, one whose chosen logits are all
+    weights = ``scale`` * s, with ``renormalise`` divided by the sum of the row's chosen s. Keys of NaN and -inf
+    are the lowest, below every number (masks of the type's lowest value go before them); a row that holds one (or +inf under softmax) has NaN weights, one whose chosen logits are all
     -inf zeros. E <= 1024, k <= 32, groups <= 64."""
     if logits.dim() != 2 or logits.dtype not in TYPES:
         raise ValueError("route: logits must be [T, E] float32, bfloat16 or float16")
