@@ -97,6 +97,7 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_s
         if bias.dtype != torch.float32 or tuple(bias.shape) != (E,) or bias.device != logits.device:
             raise ValueError(f"route: bias must be float32 [{E}] on {logits.device}")
         bias = bias.detach().contiguous()
+    fp8.refuse_dual("route", logits)
     _lib.require_gpu(logits)
     if logits.stride(1) != 1 and E > 1:
         logits = logits.contiguous()
@@ -206,6 +207,7 @@ def combine(y, weights, plan):
         raise ValueError(f"combine: y must have the plan's {plan.order.numel()} rows")
     if weights.dtype != torch.float32 or weights.shape != plan.position.shape or weights.device != y.device:
         raise ValueError(f"combine: weights must be float32 {list(plan.position.shape)} on {y.device}")
+    fp8.refuse_dual("combine", y, weights)
     _lib.require_gpu(y)
     y, weights = y.contiguous(), weights.contiguous()
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._lib import NerfHipError, enqueue, ptr
@@ -83,6 +84,13 @@ def quantize_weight(w):
     return Fp8Weight(q, scale, K)
 
 
+def refuse_dual(who, *tensors):
+    """The kernels would drop a dual number's tangent."""
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise NerfHipError(f"{who} has no forward-mode derivative: unpack its dual inputs first")
+
+
 def launch(x, weight, M, order, slots, offsets, bias, relu, out_dtype, who):
     """The checked launch that ``linear`` and ``experts.expert_linear`` share: x [rows, K] ->
     [M, N]."""
@@ -91,6 +99,7 @@ def launch(x, weight, M, order, slots, offsets, bias, relu, out_dtype, who):
     K, N = weight.k, weight.q.shape[-2]
     if x.shape[1] != K:
         raise ValueError(f"{who}: activations have {x.shape[1]} columns, the weights {K}")
+    refuse_dual(who, x, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise NerfHipError(f"{who} has no gradient: detach its inputs or run it under torch.no_grad()")
     out_dtype = out_dtype or x.dtype
