@@ -82,7 +82,7 @@ class HipAdam(torch.optim.Adam):
         if not torch.is_tensor(lr) or lr.device != self._count.device or lr.dtype != torch.float32:
             # a float set by someone else, or a tensor of a state dict loaded to another device: the
             # kernel reads one float32 of this device
-            lr = g["lr"] = torch.tensor(float(lr), device=self._count.device)
+            lr = g["lr"] = torch.tensor(float(lr), device=self._count.device, dtype=torch.float32)
         rows, changed = [], [self._count]
         missing = [p for p in g["params"] if p.grad is None]
         if missing and len(missing) != len(g["params"]):

@@ -188,7 +188,7 @@ class HipMuon(torch.optim.Optimizer):
         lr = g["lr"]
         if not torch.is_tensor(lr) or lr.device != self._lr.device or lr.dtype != torch.float32:
             # a float set by someone else, or a tensor of a state dict loaded to another device
-            lr = g["lr"] = torch.tensor(float(lr), device=self._lr.device)
+            lr = g["lr"] = torch.tensor(float(lr), device=self._lr.device, dtype=torch.float32)
         buffers = []
         for p in g["params"]:
             st = self.state[p]
