@@ -77,6 +77,20 @@ def _float32_matrix(t, shape, what):
         raise ValueError(f"muon_update: {what} must be contiguous float32 matrices of their parameter's shape")
 
 
+def _refuse_shared(spans):
+    """Memory (start, end, whether it is written): what is written may not be another's, too."""
+    spans.sort()
+    if all(a[1] <= b[0] for a, b in zip(spans, spans[1:])):
+        return
+    any_end = written_end = 0
+    for start, end, write in spans:
+        if start < (any_end if write else written_end):
+            raise ValueError("muon_update: a matrix or momentum shares memory with another one or with a gradient")
+        any_end = max(any_end, end)
+        if write:
+            written_end = max(written_end, end)
+
+
 @torch.no_grad()
 def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=STEPS, eps=EPS,
                 clip=None):
@@ -84,7 +98,8 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     buf = momentum * buf + g; u = g + momentum * buf (``nesterov``; else buf);
     p = p * (1 - lr * weight_decay) - lr * sqrt(max(1, m / n)) * orthogonalize(u).
     ``lr``: a number, or one float32 on the device (then the step can be captured and replayed with another
-    one). ``clip``: gradients clamped to [-clip, clip] on their way in (the gradients themselves stay)."""
+    one). ``clip``: gradients clamped to [-clip, clip] on their way in (the gradients themselves stay). No two
+    of params and momenta may share memory, nor a gradient with them."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_update: params, grads and momenta must be lists of one length")
@@ -93,7 +108,7 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
         raise ValueError("muon_update: momentum must be in [0, 1), eps positive, weight_decay >= 0")
     if clip is not None and not clip >= 0:
         raise ValueError("muon_update: clip must be None or >= 0")
-    seen, groups = set(), []
+    spans, groups = [], []
     for p, g, b in zip(params, grads, momenta):
         _float32_matrix(p, None, "params")
         _float32_matrix(g, p.shape, "grads")
@@ -104,11 +119,10 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
             raise ValueError("muon_update: sides up to 2^20")
         if p.numel() == 0:
             continue
-        for t in (p, b):
-            if t.data_ptr() in seen:
-                raise ValueError("muon_update: a matrix (or momentum) is there twice")
-            seen.add(t.data_ptr())
-        groups.append(_Group(ptr(p), ptr(g), ptr(b), *p.shape, 1, 0, 0))
+        size, at_p, at_g, at_b = 4 * p.numel(), ptr(p), ptr(g), ptr(b)
+        spans += (at_p, at_p + size, True), (at_b, at_b + size, True), (at_g, at_g + size, False)
+        groups.append(_Group(at_p, at_g, at_b, *p.shape, 1, 0, 0))
+    _refuse_shared(spans)
     dev_lr = torch.is_tensor(lr)
     if dev_lr and (lr.dtype != torch.float32 or lr.numel() != 1 or (params and lr.device != params[0].device)):
         raise ValueError("muon_update: a tensor lr must be one float32 on the parameters' device")
