@@ -644,8 +644,10 @@ int nerf_expert_plan(const int* experts, int64_t n, int E, int* order, int* posi
 
 /* nerf_expert_combine: out[t] = sum_j weights[t][j] y[position[t][j]] (y
  *   [rows][N], out [T][N] of one type, contiguous; positions outside of
- *   [0, rows) add nothing). _backward: d y [rows][N] (zeros where order is -1)
- *   and d weights [T][k]; either may be NULL. */
+ *   [0, rows) add nothing). _backward: d y [rows][N] and d weights [T][k];
+ *   either may be NULL. Row p of d y comes from slot order[p] where that slot's
+ *   position is p, and is zero elsewhere (order and position as
+ *   nerf_expert_plan writes them; slots may be taken out of position since). */
 int nerf_expert_combine(const void* y, int type, int64_t rows, int64_t N, const float* weights,
                         const int* position, int64_t T, int k, void* out, nerf_stream_t stream);
 int nerf_expert_combine_backward(const void* y, int type, int64_t rows, int64_t N,

@@ -838,8 +838,9 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, i
 }
 
 // d y[position[t][j]] = w[t][j] d out[t], d w[t][j] = d out[t] . y[position[t][j]]: one wave for
-// each t reads d out[t] once; the rows behind the last expert's get zeros. Bound by HBM: 168 MB in 37.5 us
-// (131072 rows of 256), 4.5 TB/s.
+// each t reads d out[t] once. A row is written by the slot that order and position both name for it, else
+// with zeros (behind the last expert's rows, or a slot taken out of position): always, and once. Bound by HBM:
+// 168 MB in 37.5 us (131072 rows of 256), 4.5 TB/s.
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restrict__ y, int64_t rows, int64_t N,
                                                                const float* __restrict__ w, const int* __restrict__ position,
@@ -853,6 +854,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restri
     for (int j = 0; j < k; ++j) {
       const int p = position[t * k + j];
       const bool live = p >= 0 && p < rows;
+      const bool own = live && dy && order[p] == t * k + j;
       const float c = w[t * k + j];
       float dot = 0.0f;
       if (live) {
@@ -864,7 +866,7 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restri
 #pragma unroll
             for (int q = 0; q < W; ++q) dot = __builtin_fmaf(d[q], v[q], dot);
           }
-          if (dy) {
+          if (own) {
 #pragma unroll
             for (int q = 0; q < W; ++q) v[q] = c * d[q];
             store_w<T, W>(dy + p * N + n, v, N - n, VEC);
@@ -878,9 +880,13 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restri
     }
   }
   if (dy) {
-    for (int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); p < rows; p += waves)
-      if (order[p] < 0)
-        for (int64_t n = lane; n < N; n += 64) dy[p * N + n] = (T)0.0f;
+    for (int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); p < rows; p += waves) {
+      const int s = order[p];
+      if (s < 0 || s >= Tn * k || position[s] != p) {
+        const float none[W] = {};
+        for (int64_t n = lane * W; n < N; n += 64 * W) store_w<T, W>(dy + p * N + n, none, N - n, VEC);
+      }
+    }
   }
 }
 

@@ -199,7 +199,8 @@ class _CombineFn(torch.autograd.Function):
 
 def combine(y, weights, plan):
     """out [T, N] in y's type: out[t] = sum_j weights[t, j] * y[plan.position[t, j]], added in float32 in the
-    order of j. y [n, N] float32, bfloat16 or float16, weights float32 [T, k]; differentiable in both."""
+    order of j. y [n, N] float32, bfloat16 or float16, weights float32 [T, k]; differentiable in both. A slot
+    whose position was set to -1 since (over a capacity, say) has no part; no two slots may have one position."""
     if y.dim() != 2 or y.dtype not in TYPES:
         raise ValueError("combine: y must be [n, N] float32, bfloat16 or float16")
     _check_plan(plan, y.device, "combine")
