@@ -697,6 +697,8 @@ int nerf_fp8_quantize_weight(const void* w, int type, int64_t stack_stride, int6
  *   clip >= 0: g is clamped to [-clip, clip] on its way in. lr_device (one
  *   float on the device) goes before lr where it is not NULL. Update: FP32.
  *   A matrix with a value that is not finite becomes NaN; zeros stay zeros.
+ *   No out or momentum may share memory with another one or with a g.
+ *   eps > 0.
  *   Workspace 16-byte aligned. */
 typedef struct NerfMuonGroup {
   void* out;               /* [count][m][n], matrices out_stride elements apart */

@@ -420,7 +420,7 @@ __global__ __launch_bounds__(S::NT) void product_kernel(const LinearArgs a, int 
         if (kb < a.KB && nb < a.NB) bytes[q] = (char)ws[nb * a.KB + kb];
       }
     };
-    tile_steps<S, kLoads>(a.KB, plan, load, chunk, scales);
+    tile_steps<S, kLoads>(a.KB, plan, load, chunk, scales, [] {});
   }
   float bias[4 * S::TN] = {};
   if (!none) load_bias<S>(a, p, eb, n0, bias);

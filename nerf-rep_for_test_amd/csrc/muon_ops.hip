@@ -11,6 +11,10 @@
 // as hi + lo FP16, x = hi + lo to 22 bits, three terms in FP32 accumulators. The bounds
 // above let X be held times S (a power of two near sqrt(r c), at most 2^15), A times 2^15
 // and B times 2^14, so lo parts stay clear of FP16's least numbers and nothing overflows.
+// Where |u| is small beside eps, X starts at t = |u| / (|u| + eps) and grows by a = 3.4445 a step at
+// most: it is held times S 2^j with the largest j that keeps t a^k 2^j within the same bound, from t, on the
+// device, for each matrix and step (grown_shift; j is 0 from t = 0.6 on). Without it X's FP16 parts ran
+// out of bits (relative errors of 2e-5 at t = 1e-3, all of it at 1e-9).
 // The three products of a step are one launch each over all matrices. A and B are
 // symmetric: only tiles on and below the diagonal are computed and each is stored twice.
 // Large matrices are bound by the matrix cores (B X for two of 2048 x 4096 and one of 2048 x 2048: 234 us,
@@ -31,6 +35,11 @@ constexpr float kA = 3.4445f, kB = -4.7750f, kC = 2.0315f;
 constexpr float kScaleA = 32768.0f, kScaleB = 16384.0f;
 constexpr int kMaxGroups = 32;    // stacks of equal matrices in one launch
 constexpr int kNormBlocks = 512;  // partial sums of one matrix's norm, at most
+// .. and behind them t, as a float. (128 bytes, a cache line: rows of the buffers that follow keep to lines, 2430 us
+// against 3010 for the large matrices)
+constexpr int kNormSlots = kNormBlocks + 16;
+constexpr float kBound = 1.2024f; // singular values of X
+constexpr int kMaxShift = 110;    // (1 / (S 2^j) stays a normal number)
 
 struct Group {
   void* out;           // parameters (FP32) or results, [count] matrices out_stride apart
@@ -38,10 +47,10 @@ struct Group {
   float* buf;          // momentum, contiguous, or null
   int64_t out_stride, g_stride;
   char* work;          // per matrix: Xs, Xt, Xt', A, B (split rows)
-  double* norm;        // [count][kNormBlocks]
+  double* norm;        // [count][kNormSlots]
   int m, n, r, c, count;
   int norm_blocks;
-  float s;             // X's scale
+  float s;             // S of X's scale S 2^j
   float adjust;        // sqrt(max(1, m / n))
 };
 
@@ -80,6 +89,17 @@ __device__ __forceinline__ int find_group(const Batch& b, int& blk) {
     if (k + step <= b.count - 1 && blk >= b.end[k + step - 1]) k += step;
   blk -= k ? b.end[k - 1] : 0;
   return k;
+}
+
+// j of a matrix whose singular values are t grow at most (grow = a^k: infinity for large k).
+__device__ __forceinline__ int grown_shift(float t, float grow) {
+  const float m = fminf(t * grow, kBound) * (1.0f / kBound);   // (0 inf, NaN: kBound)
+  int e;
+  __builtin_frexpf(m, &e);
+  return e > 0 ? 0 : (e < -kMaxShift ? kMaxShift : -e);
+}
+__device__ __forceinline__ float size_of(const Group& g, int i) {
+  return *(const float*)(g.norm + (int64_t)i * kNormSlots + kNormBlocks);
 }
 
 struct HiLo {
@@ -180,7 +200,7 @@ __global__ __launch_bounds__(256) void muon_norm_kernel(const Batch b) {
   __shared__ double w[4];
   if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) g.norm[(int64_t)i * kNormBlocks + part] = (w[0] + w[1]) + (w[2] + w[3]);
+  if (threadIdx.x == 0) g.norm[(int64_t)i * kNormSlots + part] = (w[0] + w[1]) + (w[2] + w[3]);
 }
 
 __device__ __forceinline__ void put8(char* row, int k, const HiLo (&v)[8]) {   // columns k .. k + 8 of a split row
@@ -205,11 +225,15 @@ __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
   const int tn = (g.n + 63) / 64, tm = (g.m + 63) / 64;
   const int i = blk / (tm * tn), t = blk - i * tm * tn, m0 = t / tn * 64, n0 = t % tn * 64;
   double sum = 0.0;
-  for (int k = threadIdx.x; k < g.norm_blocks; k += 256) sum += g.norm[(int64_t)i * kNormBlocks + k];
+  for (int k = threadIdx.x; k < g.norm_blocks; k += 256) sum += g.norm[(int64_t)i * kNormSlots + k];
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = sum;
   __syncthreads();
-  const float inv = (float)((double)g.s / (__builtin_sqrt((wsum[0] + wsum[1]) + (wsum[2] + wsum[3])) + (double)b.eps));
+  const double norm = __builtin_sqrt((wsum[0] + wsum[1]) + (wsum[2] + wsum[3]));
+  const float size0 = (float)(norm / (norm + (double)b.eps));
+  if (t == 0 && threadIdx.x == 0) *(float*)(g.norm + (int64_t)i * kNormSlots + kNormBlocks) = size0;
+  // (64 bits: beyond 32 for a small |u| or eps)
+  const double inv = __builtin_ldexp((double)g.s, grown_shift(size0, 1.0f)) / (norm + (double)b.eps);
   const int64_t size = (int64_t)g.m * g.n;
   const char* src = (const char*)g.g + i * g.g_stride * (b.type == NERF_F32 ? 4 : 2);
   const float* buf = g.buf ? g.buf + i * size : nullptr;
@@ -228,7 +252,7 @@ __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
   for (int u = 0; u < 16; ++u) {
     float x = clipped(v[u], b.clip);
     if (buf) x = b.nesterov ? x + b.mu * mo[u] : mo[u];
-    tile[u * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = x * inv;
+    tile[u * 4 + (threadIdx.x >> 6)][threadIdx.x & 63] = (float)((double)x * inv);
   }
   __syncthreads();
   const Work w = work_of(g, i);
@@ -279,11 +303,12 @@ __device__ __forceinline__ void finish(T* at, const float (&f)[8], int room, boo
 
 enum { kStepA = 0, kStepB = 1, kStepX = 2, kStepLast = 3 };
 
-// One product of a step for every matrix of the batch; flip: which of the two transposes is read. (Two
+// One product of a step for every matrix of the batch; flip: which of the two transposes is read; grow: a^k of
+// step k. (Two
 // waves on a SIMD: the accumulators stay in place in the VGPRs; with the whole register file the compiler
 // put them into AGPRs and moved them every step, 2690 us against 2520 for the large matrices.)
 template <class S, int STEP, class T>
-__global__ __launch_bounds__(S::NT, 2) void muon_product_kernel(const Batch bt, int flip) {
+__global__ __launch_bounds__(S::NT, 2) void muon_product_kernel(const Batch bt, int flip, float grow) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   constexpr int TM = S::TM, TN = S::TN;
   int blk = blockIdx.x;
@@ -309,6 +334,7 @@ __global__ __launch_bounds__(S::NT, 2) void muon_product_kernel(const Batch bt, 
   const int kdim = STEP == kStepA ? g.c : g.r;
   const int64_t ld = row_bytes(kdim);
   const int m0 = mt * S::BM, n0 = nt * S::BN, steps = (kdim + 31) / 32;
+  const float size = STEP == kStepB ? 0.0f : size_of(g, i);   // (on its way during the product)
   TileProduct<S> p;
   p.init(M, ld, m0, rows, N, ld, n0, cols);
   using P = TileProduct<S>;
@@ -320,13 +346,20 @@ __global__ __launch_bounds__(S::NT, 2) void muon_product_kernel(const Batch bt, 
         const char* stage = lds + k % S::NS * S::kStage;
         p.chunk(stage, stage + S::BM * 128, kLoads, part);
       },
-      [](int) {});
+      [](int) {},
+      // (its wait here, behind the first loads: a scalar load still open in the loop would make every wait for an
+      // operand from LDS one for all of them)
+      [&] { asm volatile("" ::"s"(size)); });
   char* to = STEP == kStepA ? w.a : (STEP == kStepB ? w.b : w.xs);
   const char* add = STEP == kStepB ? w.a : w.xs;   // the term beside the product
   const int64_t lto = row_bytes(cols);
   constexpr int PITCH = S::BM + 4;   // LDS row of the transposed tile, words
   unsigned* tr = (unsigned*)lds;
-  const float unscale = STEP == kStepA ? kScaleA / (g.s * g.s) : 1.0f;
+  // X comes times g.s 2^j and goes on times g.s 2^(j + next) (A of a large j is nothing beside 1: 0)
+  const int j = STEP == kStepB ? 0 : grown_shift(size, grow);
+  const float unscale = STEP == kStepA ? __builtin_ldexpf(kScaleA / (g.s * g.s), -2 * j) : 1.0f;
+  const float next = STEP == kStepX ? __builtin_ldexpf(1.0f, grown_shift(size, grow * kA) - j) : 1.0f;
+  const float beside_x = kA * next, acc_x = 1.0f / kScaleB * next, unscale_x = __builtin_ldexpf(1.0f / g.s, -j);
   const float lr = STEP == kStepLast ? (bt.lr_dev ? *bt.lr_dev : bt.lr) : 0.0f;
   const float keep = 1.0f - lr * bt.decay, rate = lr * g.adjust;
   const bool tall = g.m > g.n, once = STEP < kStepX && mt == nt;   // (on the diagonal: no transposed tile)
@@ -356,13 +389,13 @@ __global__ __launch_bounds__(S::NT, 2) void muon_product_kernel(const Batch bt, 
           const float beside = (float)ah[e] + (float)al[e];
           if (STEP == kStepA) x = acc * unscale;
           if (STEP == kStepB) x = kB * (kScaleB / kScaleA) * beside + kC * (kScaleB / (kScaleA * kScaleA)) * acc;
-          if (STEP >= kStepX) x = kA * beside + acc * (1.0f / kScaleB);
+          if (STEP >= kStepX) x = beside_x * beside + acc_x * acc;
           f[e] = ALL || nn + e < cols ? x : 0.0f;
           if (STEP != kStepLast) v[e] = split(f[e]);
         }
         if (STEP == kStepLast) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= 1.0f / g.s;
+          for (int e = 0; e < 8; ++e) f[e] *= unscale_x;
           if (tall) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) tr[(nl + e) * PITCH + ml] = __float_as_uint(f[e]);
@@ -422,7 +455,7 @@ int check_group(const NerfMuonGroup& g, bool update) {
 
 int64_t group_bytes(const NerfMuonGroup& g) {
   const int r = (int)(g.m < g.n ? g.m : g.n), c = (int)(g.m < g.n ? g.n : g.m);
-  return g.count * (work_bytes(r, c) + (int64_t)kNormBlocks * 8);
+  return g.count * (work_bytes(r, c) + (int64_t)kNormSlots * 8);
 }
 
 int64_t count_tiles(const Group& g, int bm, int bn, bool square) {
@@ -437,7 +470,7 @@ constexpr size_t lds_bytes() {
 }
 
 template <class S, int STEP, class T>
-int launch_step(Batch& b, int flip, hipStream_t st) {
+int launch_step(Batch& b, int flip, float grow, hipStream_t st) {
   int64_t end = 0;
   for (int k = 0; k < b.count; ++k) {
     end += count_tiles(b.g[k], S::BM, S::BN, STEP < kStepX);
@@ -445,21 +478,22 @@ int launch_step(Batch& b, int flip, hipStream_t st) {
     b.end[k] = (int)end;
   }
   hipLaunchKernelGGL((muon_product_kernel<S, STEP, T>), dim3((unsigned)end), dim3(S::NT), lds_bytes<S>(),
-                     st, b, flip);
+                     st, b, flip, grow);
   return check_launch("nerf_muon");
 }
 
 template <class S>
 int run_steps(Batch& b, int steps, bool update, hipStream_t st) {
-  for (int k = 0; k < steps; ++k) {
+  float grow = 1.0f;
+  for (int k = 0; k < steps; ++k, grow *= kA) {
     const int flip = k & 1;
-    if (const int rc = launch_step<S, kStepA, float>(b, flip, st)) return rc;
-    if (const int rc = launch_step<S, kStepB, float>(b, flip, st)) return rc;
+    if (const int rc = launch_step<S, kStepA, float>(b, flip, grow, st)) return rc;
+    if (const int rc = launch_step<S, kStepB, float>(b, flip, grow, st)) return rc;
     int rc;
-    if (k + 1 < steps) rc = launch_step<S, kStepX, float>(b, flip, st);
-    else if (update || b.type == NERF_F32) rc = launch_step<S, kStepLast, float>(b, flip, st);
-    else if (b.type == NERF_BF16) rc = launch_step<S, kStepLast, bf16>(b, flip, st);
-    else rc = launch_step<S, kStepLast, f16>(b, flip, st);
+    if (k + 1 < steps) rc = launch_step<S, kStepX, float>(b, flip, grow, st);
+    else if (update || b.type == NERF_F32) rc = launch_step<S, kStepLast, float>(b, flip, grow, st);
+    else if (b.type == NERF_BF16) rc = launch_step<S, kStepLast, bf16>(b, flip, grow, st);
+    else rc = launch_step<S, kStepLast, f16>(b, flip, grow, st);
     if (rc) return rc;
   }
   return 0;
@@ -484,6 +518,7 @@ int nerf_muon(const NerfMuonGroup* groups, int n, const NerfMuonOptions* o, void
   NERF_REQUIRE(n >= 1 && o->steps >= 1 && o->type >= NERF_F32 && o->type <= NERF_F16 &&
                    (!o->update || o->type == NERF_F32),
                "nerf_muon: bad count, steps or type");
+  NERF_REQUIRE(o->eps > 0.0f && o->eps <= 3.402823466e+38f, "nerf_muon: eps must be positive and finite");
   for (int k = 0; k < n; ++k)
     if (const int rc = check_group(groups[k], o->update != 0)) return rc;
   NERF_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= nerf_muon_workspace(groups, n),
@@ -523,7 +558,7 @@ int nerf_muon(const NerfMuonGroup* groups, int n, const NerfMuonOptions* o, void
       g.s = (float)(1 << e);
       g.adjust = s.m > s.n ? (float)__builtin_sqrt((double)s.m / (double)s.n) : 1.0f;
       g.norm = (double*)at;
-      at += g.count * (int64_t)kNormBlocks * 8;
+      at += g.count * (int64_t)kNormSlots * 8;
       g.work = at;
       at += g.count * work_bytes(g.r, g.c);
       end += (int64_t)g.count * g.norm_blocks;

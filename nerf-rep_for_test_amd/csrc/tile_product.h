@@ -319,9 +319,9 @@ __device__ __forceinline__ void stage_ready() {
 // The steps k = 0 .. n of a product over S::NS stages. plan(k): what the loads of chunk k into stage
 // k % NS need (nothing that counts behind the last chunk); load(plan, q): one of them, q = 0 .. kLoads - 1 in
 // each wave; chunk(k, part): its products, with part(0) .. part(kLoads - 1) between them. before(k) runs
-// ahead of the barrier behind which chunk k is in LDS.
-template <class S, int kLoads, class PLAN, class LOAD, class CHUNK, class BEFORE>
-__device__ __forceinline__ void tile_steps(int n, PLAN plan, LOAD load, CHUNK chunk, BEFORE before) {
+// ahead of the barrier behind which chunk k is in LDS; started() when the first stages' loads are on their way.
+template <class S, int kLoads, class PLAN, class LOAD, class CHUNK, class BEFORE, class STARTED>
+__device__ __forceinline__ void tile_steps(int n, PLAN plan, LOAD load, CHUNK chunk, BEFORE before, STARTED started) {
   constexpr int NS = S::NS;
 #pragma unroll
   for (int k = 0; k < NS - 1; ++k) {
@@ -329,6 +329,7 @@ __device__ __forceinline__ void tile_steps(int n, PLAN plan, LOAD load, CHUNK ch
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) load(l, q);
   }
+  started();
   for (int k = 0; k < n; ++k) {
     before(k);
     const auto l = plan(k + NS - 1);

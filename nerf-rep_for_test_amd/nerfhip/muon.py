@@ -48,17 +48,22 @@ def _check_steps(steps):
     return int(steps)
 
 
+def _is_eps(eps):
+    """Positive and finite as the 32-bit number that the kernels take."""
+    return 0.0 < ctypes.c_float(eps).value < float("inf")
+
+
 @torch.no_grad()
 def orthogonalize(g, steps=STEPS, eps=EPS):
     """Newton-Schulz orthogonalisation of a matrix [m, n] or a stack [.., m, n] (float32, bfloat16, float16;
     result in the same type): X = g / (|g| + eps), then ``steps`` times X = a X + (b A + c A A) X with
-    A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315); singular values end near 1. Sums, norms and products hold
-    float32 accuracy whatever the type. A matrix with a value that is not finite becomes NaN. No gradient."""
+    A = X X^T, (a, b, c) = (3.4445, -4.7750, 2.0315); singular values end near 1 where |g| is not far below eps.
+    Sums, norms and products hold float32 accuracy whatever the type and |g|. A matrix with a value that is not finite becomes NaN. No gradient."""
     if g.dim() < 2 or g.dtype not in TYPES:
         raise ValueError("orthogonalize: g must be [.., m, n] float32, bfloat16 or float16")
     steps = _check_steps(steps)
-    if not 0.0 < eps < float("inf"):
-        raise ValueError("orthogonalize: eps must be positive")
+    if not _is_eps(eps):
+        raise ValueError("orthogonalize: eps must be a positive 32-bit number")
     m, n = g.shape[-2:]
     if max(m, n) > 1 << 20:
         raise ValueError("orthogonalize: sides up to 2^20")
@@ -104,7 +109,7 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon_update: params, grads and momenta must be lists of one length")
     steps = _check_steps(steps)
-    if not 0.0 <= momentum < 1.0 or not 0.0 < eps < float("inf") or not 0.0 <= weight_decay < float("inf"):
+    if not 0.0 <= momentum < 1.0 or not _is_eps(eps) or not 0.0 <= weight_decay < float("inf"):
         raise ValueError("muon_update: momentum must be in [0, 1), eps positive, weight_decay >= 0")
     if clip is not None and not clip >= 0:
         raise ValueError("muon_update: clip must be None or >= 0")
