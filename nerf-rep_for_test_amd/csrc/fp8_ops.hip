@@ -242,7 +242,7 @@ __device__ __forceinline__ float relu_of(float v) { return v < 0.0f ? 0.0f : v; 
 // (8192 x 8192 x 8192: 455 us, 2.4 PFLOP/s; the library's own 8-bit product reaches 2.5 to 2.7), those of
 // experts by their short rows: 32768 of 2048 in 242 us, 1.1 PFLOP/s, a third of it starts and ends of tiles.
 
-// Workgroup -> (expert, row tile): experts' row tiles one after another. Wave 0 sums the
+// Workgroup -> (expert, row tile): experts' row tiles one after another. Every wave sums the
 // experts' tile counts 64 at a time until the tile is met.
 template <int BM>
 __device__ __forceinline__ bool find_tile(const LinearArgs& a, int tile, int& e, int64_t& m0, int64_t& hi) {
@@ -514,11 +514,44 @@ __global__ __launch_bounds__(S::NT) void resident_kernel(const LinearArgs a, int
 
 // ---------------------------------------------------------------- skinny form
 
+// Tile `tile` of the tiles of 16 rows behind each expert's first: a lane counts those of a run of experts.
+__device__ __forceinline__ bool find_further(const LinearArgs& a, int tile, int& e, int64_t& m0, int64_t& hi) {
+  const int lane = threadIdx.x & 63, n = a.offsets ? a.E + 1 : 1, per = (n + 63) / 64;
+  const auto tiles = [&](int at) {
+    int64_t lo = 0, end = 0;
+    if (at < n) expert_rows(a, at, lo, end);
+    return end > lo ? (int)((end - lo - 1) / 16) : 0;
+  };
+  int mine = 0;
+#pragma unroll 4
+  for (int i = 0; i < per; ++i) mine += tiles(lane * per + i);
+  int sum = mine;
+  for (int d = 1; d < 64; d *= 2) {
+    const int o = __shfl_up(sum, d);
+    if (lane >= d) sum += o;
+  }
+  const unsigned long long met = __ballot(sum > tile);
+  if (!met) return false;
+  const int at = __builtin_ctzll(met);
+  int left = tile - __builtin_amdgcn_readlane(sum - mine, at);
+  e = at * per;
+  for (int c; (c = tiles(e)) <= left; ++e) left -= c;   // (ends: that lane counted more than `left`)
+  e = __builtin_amdgcn_readfirstlane(e);
+  expert_rows(a, e, m0, hi);
+  m0 += 16 * (int64_t)(__builtin_amdgcn_readfirstlane(left) + 1);
+  return true;
+}
+
 // Few rows for each weight matrix: bound by the weights' bytes. A workgroup of 8 waves
-// takes 16 TN weight rows; the waves share the blocks of K between them, U at a time (all
-// of their loads in flight), read the weights straight into the matrix operands (16 rows x
-// 128 B lines, no LDS) and quantise the activations in registers (a row's block lies in 4
-// lanes), so one launch reads each weight once. The 8 partial sums are added in wave order.
+// takes 16 rows of x (blockIdx.y: the first 16 of each expert, then the further 16s of whatever
+// experts have them) and 16 TN weight rows;
+// the waves share the blocks of K between them, U at a time (all of their loads in flight),
+// read the weights straight into the matrix operands (16 rows x 128 B lines, no LDS) and
+// quantise the activations in registers (a row's block lies in 4 lanes), so one launch
+// reads each weight once for every 16 rows. The 8 partial sums are added in wave order.
+// Rows that a gate spreads unevenly (64 experts of 1024 x 2048, 1024 rows; 256 of 512 x 1024, 4096): all on one
+// expert 30 and 43 us (one workgroup walking them all: 415 and 990), at random 40 and 52 (48 and 47), evenly 30
+// and 41 (28 and 35: the further 16s' workgroups start and find nothing).
 // 4096 x 4096 for one row in 7.1 us (2.4 TB/s: its start and end are half of that), 64 experts of
 // 1024 x 2048 with 96 rows in 21 us (5 TB/s).
 template <class T, class O, int TN, bool VEC>
@@ -527,10 +560,15 @@ __global__ __launch_bounds__(512) void skinny_kernel(const LinearArgs a) {
   __shared__ float part[W][TN][16][17];
   const int t = threadIdx.x, w = t >> 6, lane = t & 63, g = lane >> 4, r = lane & 15;
   const int64_t n0 = (int64_t)blockIdx.x * 16 * TN;
-  const int e = blockIdx.y;
-  int64_t lo, hi;
-  expert_rows(a, e, lo, hi);
-  if (lo >= hi) return;
+  const int firsts = a.offsets ? a.E + 1 : 1;
+  int e = blockIdx.y;
+  int64_t m0, hi;
+  if (e < firsts) {
+    expert_rows(a, e, m0, hi);
+    if (m0 >= hi) return;
+  } else if (!find_further(a, e - firsts, e, m0, hi)) {
+    return;
+  }
   const bool none = a.offsets && e == a.E;
   const int eb = none ? 0 : e;
   const unsigned char* wrow[TN];
@@ -540,83 +578,80 @@ __global__ __launch_bounds__(512) void skinny_kernel(const LinearArgs a) {
     const int64_t n = n0 + 16 * j + r;
     wrow[j] = a.wq + ((int64_t)eb * a.N + (n < a.N ? n : a.N - 1)) * a.KB * 128 + g * 16;
   }
-  for (int64_t m0 = lo; m0 < hi; m0 += 16) {
-    f32x4 acc[TN];
+  f32x4 acc[TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[j] = f32x4(0.0f);
-    const int64_t src = source_row(a.order, a.div, a.x_rows, m0 + r < hi ? m0 + r : hi - 1);
-    const T* xrow = src < 0 ? nullptr : (const T*)a.x + src * a.ldx;
-    for (int k0 = w; k0 < a.KB && !none; k0 += W * U) {
-      i32x4 wf[U][TN][2];
-      int sn[U];
-      T x[U][2][16];
+  for (int j = 0; j < TN; ++j) acc[j] = f32x4(0.0f);
+  const int64_t src = source_row(a.order, a.div, a.x_rows, m0 + r < hi ? m0 + r : hi - 1);
+  const T* xrow = src < 0 ? nullptr : (const T*)a.x + src * a.ldx;
+  for (int k0 = w; k0 < a.KB && !none; k0 += W * U) {
+    i32x4 wf[U][TN][2];
+    int sn[U];
+    T x[U][2][16];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {   // (blocks behind the last one: the last one again, not used)
-        const int64_t k = k0 + u * W < a.KB ? k0 + u * W : a.KB - 1;
+    for (int u = 0; u < U; ++u) {   // (blocks behind the last one: the last one again, not used)
+      const int64_t k = k0 + u * W < a.KB ? k0 + u * W : a.KB - 1;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        wf[u][j][0] = *(const i32x4*)(wrow[j] + k * 128);
+        wf[u][j][1] = *(const i32x4*)(wrow[j] + k * 128 + 64);
+      }
+      sn[u] = ws[k];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 16; c += 8) {
+          T v[8] = {};
+          if (xrow) load_raw<T, VEC>(v, xrow, k * 128 + h * 64 + g * 16 + c, a.K);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) x[u][h][c + q] = v[q];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[2][16];
+      unsigned top = 0;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        f[c >> 4][c & 15] = (float)x[u][c >> 4][c & 15];
+        top = max(top, abs_bits(f[c >> 4][c & 15]));
+      }
+      top = max4(top);
+      const int sc = block_scale(top), ex = 127 - sc;
+      i32x8 xf;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float* v = &f[c >> 2][(c & 3) * 4];
+        xf[c] = pack4(__builtin_ldexpf(v[0], ex), __builtin_ldexpf(v[1], ex), __builtin_ldexpf(v[2], ex),
+                      __builtin_ldexpf(v[3], ex));
+      }
+      if (k0 + u * W < a.KB) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-          wf[u][j][0] = *(const i32x4*)(wrow[j] + k * 128);
-          wf[u][j][1] = *(const i32x4*)(wrow[j] + k * 128 + 64);
-        }
-        sn[u] = ws[k];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < 16; c += 8) {
-            T v[8] = {};
-            if (xrow) load_raw<T, VEC>(v, xrow, k * 128 + h * 64 + g * 16 + c, a.K);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[u][h][c + q] = v[q];
-          }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float f[2][16];
-        unsigned top = 0;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          f[c >> 4][c & 15] = (float)x[u][c >> 4][c & 15];
-          top = max(top, abs_bits(f[c >> 4][c & 15]));
-        }
-        top = max4(top);
-        const int sc = block_scale(top), ex = 127 - sc;
-        i32x8 xf;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float* v = &f[c >> 2][(c & 3) * 4];
-          xf[c] = pack4(__builtin_ldexpf(v[0], ex), __builtin_ldexpf(v[1], ex), __builtin_ldexpf(v[2], ex),
-                        __builtin_ldexpf(v[3], ex));
-        }
-        if (k0 + u * W < a.KB) {
-#pragma unroll
-          for (int j = 0; j < TN; ++j) {
-            const i32x8 wj = __builtin_shufflevector(wf[u][j][0], wf[u][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
-            if constexpr (sizeof(O) == 4)
-              acc[j] = wide_block(wj, xf, sn[u], sc, acc[j]);
-            else
-              acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wj, xf, acc[j], 0, 0, 0, sn[u], 0, sc);
-          }
+          const i32x8 wj = __builtin_shufflevector(wf[u][j][0], wf[u][j][1], 0, 1, 2, 3, 4, 5, 6, 7);
+          if constexpr (sizeof(O) == 4)
+            acc[j] = wide_block(wj, xf, sn[u], sc, acc[j]);
+          else
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wj, xf, acc[j], 0, 0, 0, sn[u], 0, sc);
         }
       }
     }
+  }
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+  for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) part[w][j][r][g * 4 + c] = acc[j][c];   // [row m][column n]
-    __syncthreads();
-    for (int o = t; o < TN * 256; o += 512) {
-      const int j = (o >> 4) % TN, m = (o >> 4) / TN, c = o & 15;
-      float v = part[0][j][m][c];
+    for (int c = 0; c < 4; ++c) part[w][j][r][g * 4 + c] = acc[j][c];   // [row m][column n]
+  __syncthreads();
+  for (int o = t; o < TN * 256; o += 512) {
+    const int j = (o >> 4) % TN, m = (o >> 4) / TN, c = o & 15;
+    float v = part[0][j][m][c];
 #pragma unroll
-      for (int u = 1; u < W; ++u) v += part[u][j][m][c];
-      const int64_t row = m0 + m, n = n0 + 16 * j + c;
-      if (row < hi && n < a.N) {
-        if (a.bias && !none) v += a.bias[(int64_t)eb * a.N + n];
-        if (a.relu) v = relu_of(v);
-        ((O*)a.out)[row * a.ldo + n] = (O)v;
-      }
+    for (int u = 1; u < W; ++u) v += part[u][j][m][c];
+    const int64_t row = m0 + m, n = n0 + 16 * j + c;
+    if (row < hi && n < a.N) {
+      if (a.bias && !none) v += a.bias[(int64_t)eb * a.N + n];
+      if (a.relu) v = relu_of(v);
+      ((O*)a.out)[row * a.ldo + n] = (O)v;
     }
-    __syncthreads();
   }
 }
 
@@ -669,9 +704,10 @@ void launch_resident_out(const LinearArgs& a, int out_type, hipStream_t st) {
 template <class T, class O, int TN>
 void launch_skinny(const LinearArgs& a, hipStream_t st) {
   const bool vec = aligned16(a.x, a.ldx, sizeof(T)) && a.K % (16 / sizeof(T)) == 0;
+  // (further 16s: a matrix with r rows has (r - 1) / 16 of them, all together (M - 1) / 16 at most)
+  const int64_t tiles = (a.offsets ? a.E + 1 : 1) + (a.M - 1) / 16;
   auto* kern = vec ? skinny_kernel<T, O, TN, true> : skinny_kernel<T, O, TN, false>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(a.N, 16 * TN), (unsigned)(a.offsets ? a.E + 1 : 1)), dim3(512), 0, st,
-                     a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(a.N, 16 * TN), (unsigned)tiles), dim3(512), 0, st, a);
 }
 
 template <class T, class O>
@@ -695,8 +731,11 @@ void launch_skinny_out(const LinearArgs& a, int out_type, hipStream_t st) {
 
 // Few rows for each weight matrix: the skinny form, which takes 16 rows (one matrix operand) at a time and
 // reads the weights again for the next 16 (4096 x 4096, 16-bit rows: 32 of them 17 us, tiled 21; 48: 23
-// and 21; 16 experts of 1024 x 2048 with 256 rows: 16 and 18 us, with 512: 23 and 19).
-bool is_skinny(int64_t M, int E, bool grouped) { return grouped ? M <= 16 * (int64_t)E : M <= 32; }
+// and 21; 16 experts of 1024 x 2048 with 256 rows: 14 and 18 us, with 512: 23 and 19). However the rows are spread:
+// the host does not know it.
+bool is_skinny(int64_t M, int E, bool grouped) {
+  return grouped ? M <= 16 * (int64_t)E && E < 32767 : M <= 32;   // (2 E + 1 workgroups along y)
+}
 
 // Many rows through one small matrix: the resident form (a tile for every CU at least).
 bool is_resident(int64_t M, int64_t N, int64_t K, bool grouped) {
