@@ -927,13 +927,22 @@ RouteArgs route_args(const NerfRoute* d) {
 template <int L, int V, class T, bool VEC>
 void go_route(const RouteArgs& a, const float* dw, void* dlogits, hipStream_t st) {
   constexpr int R = 256 / L;
-  const dim3 grid((unsigned)cdiv(a.T, R));
-  if (dlogits) {
-    RouteBwdArgs b{a, dw, dlogits};
-    hipLaunchKernelGGL((route_backward_kernel<L, V, T, VEC>), grid, dim3(256), R * V * L * 4, st, b);
-  } else {
-    const size_t lds = (size_t)R * (a.groups > 1 ? a.E + 2 * a.groups : 0) * 8 + R * kMaxChoices * 4;
-    hipLaunchKernelGGL((route_kernel<L, V, T, VEC>), grid, dim3(256), lds, st, a);
+  // (a launch has less than 2^32 threads, a call up to 2^31 rows of 16 or 64 lanes each)
+  constexpr int64_t kRows = (int64_t)R << 22;
+  for (int64_t t = 0; t < a.T; t += kRows) {
+    RouteArgs p = a;
+    p.T = a.T - t < kRows ? a.T - t : kRows;
+    p.logits = (const T*)a.logits + t * a.ld;
+    p.weights = a.weights ? a.weights + t * a.k : nullptr;
+    p.experts = a.experts + t * a.k;
+    const dim3 grid((unsigned)cdiv(p.T, R));
+    if (dlogits) {
+      RouteBwdArgs b{p, dw + t * a.k, (T*)dlogits + t * a.E};
+      hipLaunchKernelGGL((route_backward_kernel<L, V, T, VEC>), grid, dim3(256), R * V * L * 4, st, b);
+    } else {
+      const size_t lds = (size_t)R * (a.groups > 1 ? a.E + 2 * a.groups : 0) * 8 + R * kMaxChoices * 4;
+      hipLaunchKernelGGL((route_kernel<L, V, T, VEC>), grid, dim3(256), lds, st, p);
+    }
   }
 }
 
