@@ -26,6 +26,10 @@ int check_launch(const char* what);
 
 __host__ __device__ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Whether one launch takes `blocks` workgroups of `threads`: of 2^32 threads or more along an axis the
+// runtime runs a part only, without an error.
+inline bool launch_fits(int64_t blocks, int threads) { return blocks >= 0 && blocks <= ((1ll << 32) - 1) / threads; }
+
 // CU count of the device a stream launches on (persistent grids: one workgroup
 // per CU), cached per device ordinal; races only write the same value. The
 // null/legacy stream resolves to the calling thread's current device.

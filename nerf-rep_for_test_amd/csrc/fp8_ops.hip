@@ -138,10 +138,10 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
 // e4m3 q [E][N][KB * 128] and scales [E][NB][KB]. One workgroup for each block.
 template <class T>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restrict__ w, int64_t sw, int64_t ldw,
-                                                              int64_t N, int64_t K, int NB, int KB,
+                                                              int64_t N, int64_t K, int NB, int KB, int64_t first,
                                                               unsigned char* __restrict__ q,
                                                               unsigned char* __restrict__ s) {
-  const int64_t id = blockIdx.x;
+  const int64_t id = first + blockIdx.x;
   const int kb = (int)(id % KB);
   const int nb = (int)(id / KB % NB);
   const int64_t e = id / KB / NB;
@@ -796,6 +796,7 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   a.q_rows = 0;
   a.gather = 0;
   if (is_skinny(d->M, d->E, d->offsets != nullptr)) {
+    NERF_REQUIRE(launch_fits(cdiv(d->N, 64), 512), "nerf_fp8_linear: too many columns");
     if (d->x_type == NERF_F32) launch_skinny_out<float>(a, d->out_type, st);
     else if (d->x_type == NERF_BF16) launch_skinny_out<bf16>(a, d->out_type, st);
     else launch_skinny_out<f16>(a, d->out_type, st);
@@ -829,7 +830,8 @@ int nerf_fp8_linear(const NerfFp8Linear* d, void* workspace, size_t workspace_by
   using SS = TileShape<Fp8, 2, 2, 2, 2>;
   using SWS = TileShape<Fp8Wide, 2, 2, 2, 2>;
   const bool small = (cdiv(d->M, 128) + (d->offsets ? (d->M < d->E ? d->M : d->E) : 0)) * cdiv(d->N, 128) <= 256;
-  NERF_REQUIRE((d->M / SS::BM + d->E + 1) * cdiv(d->N, SS::BN) < (1ll << 31), "nerf_fp8_linear: too many tiles");
+  const int side = small ? SS::BM : S::BM;   // (the largest tiles are fewer)
+  NERF_REQUIRE(launch_fits((d->M / side + d->E + 1) * cdiv(d->N, side), S::NT), "nerf_fp8_linear: too many tiles");
   if (d->x_type == NERF_F32) launch_quantize<float>(a, q, s, st);
   else if (d->x_type == NERF_BF16) launch_quantize<bf16>(a, q, s, st);
   else launch_quantize<f16>(a, q, s, st);
@@ -853,15 +855,18 @@ int nerf_fp8_quantize_weight(const void* w, int type, int64_t stack_stride, int6
   NERF_REQUIRE(KB < (1ll << 24) && NB < (1ll << 24) && E * NB * KB < (1ll << 31),
                "nerf_fp8_quantize_weight: too many blocks");
   NERF_REQUIRE((uintptr_t)q % 8 == 0, "nerf_fp8_quantize_weight: q needs 8-byte alignment");
-  const dim3 grid((unsigned)(E * NB * KB)), block(256);
+  const int64_t blocks = E * NB * KB, most = 1 << 22;   // (of one launch)
   const hipStream_t st = as_stream(stream);
+  for (int64_t first = 0; first < blocks; first += most) {
+    const dim3 grid((unsigned)(blocks - first < most ? blocks - first : most)), block(256);
 #define NERF_QW(T)                                                                                          \
   hipLaunchKernelGGL(quantize_weight_kernel<T>, grid, block, 0, st, (const T*)w, stack_stride, ldw, N, K,   \
-                     (int)NB, (int)KB, (unsigned char*)q, (unsigned char*)scale)
-  if (type == NERF_F32) NERF_QW(float);
-  else if (type == NERF_BF16) NERF_QW(bf16);
-  else NERF_QW(f16);
+                     (int)NB, (int)KB, first, (unsigned char*)q, (unsigned char*)scale)
+    if (type == NERF_F32) NERF_QW(float);
+    else if (type == NERF_BF16) NERF_QW(bf16);
+    else NERF_QW(f16);
 #undef NERF_QW
+  }
   return check_launch("nerf_fp8_quantize_weight");
 }
 

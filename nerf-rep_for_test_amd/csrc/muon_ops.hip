@@ -474,7 +474,7 @@ int launch_step(Batch& b, int flip, float grow, hipStream_t st) {
   int64_t end = 0;
   for (int k = 0; k < b.count; ++k) {
     end += count_tiles(b.g[k], S::BM, S::BN, STEP < kStepX);
-    NERF_REQUIRE(end < (1ll << 31), "nerf_muon: too many tiles");
+    NERF_REQUIRE(launch_fits(end, S::NT), "nerf_muon: too many tiles");
     b.end[k] = (int)end;
   }
   hipLaunchKernelGGL((muon_product_kernel<S, STEP, T>), dim3((unsigned)end), dim3(S::NT), lds_bytes<S>(),
@@ -566,7 +566,7 @@ int nerf_muon(const NerfMuonGroup* groups, int n, const NerfMuonOptions* o, void
       tiles += g.count * cdiv(s.m, 64) * cdiv(s.n, 64);
       split_end[k] = tiles;
       tiles64 += count_tiles(g, 128, 128, false);
-      NERF_REQUIRE(end < (1ll << 31) && tiles < (1ll << 31), "nerf_muon: too many tiles");
+      NERF_REQUIRE(launch_fits(end, 256) && launch_fits(tiles, 256), "nerf_muon: too many tiles");
     }
     hipLaunchKernelGGL(muon_norm_kernel, dim3((unsigned)end), dim3(256), 0, st, b);
     for (int k = 0; k < b.count; ++k) b.end[k] = (int)split_end[k];
