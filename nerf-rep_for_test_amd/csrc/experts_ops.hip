@@ -880,9 +880,13 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restri
     }
   }
   if (dy) {
-    for (int64_t p = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); p < rows; p += waves) {
-      const int s = order[p];
-      if (s < 0 || s >= Tn * k || position[s] != p) {
+    // 64 rows at a time are looked at by a wave, a lane each
+    for (int64_t p0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * 64; p0 < rows; p0 += waves * 64) {
+      const int64_t mine = p0 + lane;
+      const int s = mine < rows ? order[mine] : -1;
+      const bool written = s >= 0 && s < Tn * k && position[s] == mine;
+      for (unsigned long long rest = __ballot(mine < rows && !written); rest; rest &= rest - 1) {
+        const int64_t p = p0 + __builtin_ctzll(rest);
         const float none[W] = {};
         for (int64_t n = lane * W; n < N; n += 64 * W) store_w<T, W>(dy + p * N + n, none, N - n, VEC);
       }
