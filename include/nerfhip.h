@@ -664,8 +664,8 @@ int nerf_expert_combine_backward(const void* y, int type, int64_t rows, int64_t 
  *   below the largest. K <= 2^23.
  *   wq [E][N][Kp] (Kp = K rounded up to 128, zeros behind K; 16-byte aligned),
  *   ws [E][ceil(N / 128)][Kp / 128]. offsets NULL: one matrix. offsets [E + 1]:
- *   rows offsets[e] .. offsets[e + 1] take matrix e; rows behind offsets[E]
- *   become zeros. order (with slots >= 1): row i is x[order[i] / slots], a row
+ *   rows offsets[e] .. offsets[e + 1] take matrix e (offsets[0] = 0, never
+ *   falling); rows behind offsets[E] become zeros. order (with slots >= 1): row i is x[order[i] / slots], a row
  *   of zeros where that is no row of x. bias: [E][N] FP32.
  * nerf_fp8_quantize_weight: a stack of matrices [E][N][K] (rows ldw, matrices
  *   stack_stride elements apart) to wq, ws. */

@@ -401,15 +401,14 @@ __device__ __forceinline__ void choose(const RouteArgs& a, const T* row, const f
 // A chosen expert's part in the weights, r_j of the formulas: w_j = scale * r_j.
 // Renormalised: s_j / sum of the chosen s, with the chosen logits' largest taken out first
 // (m: their maximum; for sigmoid s e^-m = 1 / (e^m + e^(m - l)), m <= 0), so that scores too small
-// for 32 bits still have their ratios.
+// for 32 bits still have their ratios. In 32 bits, unlike the order: some steps of 2^-24 (5e-8 of a row's norm
+// against 64 bits where one rounding is 3e-8), as much as an FP32 sum over experts' rows adds again.
 __device__ __forceinline__ float chosen_part(const RouteArgs& a, float l, float m) {
   if (a.renorm) return a.sigmoid ? 1.0f / (expf(m) + expf(m - l)) : expf(l - m);
   return a.sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - m);
 }
 
-// Rows of L lanes, 256 / L rows in a workgroup. Reads the logits once, writes k weights and experts.
-// Bound by instructions: sorting a lane's keys and the k rounds of the choice (T = 65536: E = 64, k = 2 in
-// 11 us, 16.8 MB at 1.5 TB/s; E = 256, k = 8 in 32 us), by one row's latency for few rows (3 us for T = 1).
+// A lane's logits, -inf behind the last expert.
 template <int L, int V, class T, bool VEC>
 __device__ __forceinline__ void load_logits(const T* row, int E, int lane, float (&x)[V]) {
 #pragma unroll
@@ -431,6 +430,9 @@ __device__ __forceinline__ void load_logits(const T* row, int E, int lane, float
   }
 }
 
+// Rows of L lanes, 256 / L rows in a workgroup. Reads the logits once, writes k weights and experts.
+// Bound by instructions: sorting a lane's keys and the k rounds of the choice (T = 65536: E = 64, k = 2 in
+// 11 us, 16.8 MB at 1.5 TB/s; E = 256, k = 8 in 32 us), by one row's latency for few rows (3 us for T = 1).
 template <int L, int V, class T, bool VEC>
 __global__ __launch_bounds__(256) void route_kernel(const RouteArgs a) {
   extern __shared__ double route_lds[];
@@ -505,7 +507,7 @@ struct RouteBwdArgs {
 // d logits of a row: renormalised, only the chosen ones have a gradient:
 //   softmax: scale r_j (g_j - sum_i r_i g_i);  sigmoid: that times (1 - s_j);
 // not renormalised: softmax: p_e (scale g_e - sum_i scale g_i p_i) for every e; sigmoid: scale g s (1 - s).
-// The row is put together in LDS and written in one sweep: 33.6 MB in 13.4 us (T = 65536, E = 64), 2.5 TB/s.
+// The row is put together in LDS and written in one sweep: 33.6 MB in 12 to 13 us (T = 65536, E = 64), 2.7 TB/s.
 template <int L, int V, class T, bool VEC>
 __global__ __launch_bounds__(256) void route_backward_kernel(const RouteBwdArgs b) {
   extern __shared__ float bwd_lds[];
@@ -840,7 +842,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ y, i
 // d y[position[t][j]] = w[t][j] d out[t], d w[t][j] = d out[t] . y[position[t][j]]: one wave for
 // each t reads d out[t] once. A row is written by the slot that order and position both name for it, else
 // with zeros (behind the last expert's rows, or a slot taken out of position): always, and once. Bound by HBM:
-// 168 MB in 37.5 us (131072 rows of 256), 4.5 TB/s.
+// 168 MB in 38 us (131072 rows of 256), 4.4 TB/s.
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void combine_backward_kernel(const T* __restrict__ y, int64_t rows, int64_t N,
                                                                const float* __restrict__ w, const int* __restrict__ position,

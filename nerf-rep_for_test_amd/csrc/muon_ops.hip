@@ -17,10 +17,10 @@
 // out of bits (relative errors of 2e-5 at t = 1e-3, all of it at 1e-9).
 // The three products of a step are one launch each over all matrices. A and B are
 // symmetric: only tiles on and below the diagonal are computed and each is stored twice.
-// Large matrices are bound by the matrix cores (B X for two of 2048 x 4096 and one of 2048 x 2048: 234 us,
-// 1.1 PFLOP/s in FP16, what the library's FP16 product reaches), small ones by the latency of 17
+// Large matrices are bound by the matrix cores (B X for two of 2048 x 4096 and one of 2048 x 2048: 242 to 262 us,
+// 1.0 to 1.07 PFLOP/s in FP16; the library's FP16 product reaches 1.15), small ones by the latency of 17
 // launches (the trainer's 20 matrices: 150 us, 8 to 13 a launch), those between by HBM (32 of
-// 512 x 1024: B X moves 300 MB in 75 us).
+// 512 x 1024: B X moves 300 MB in 77 to 84 us).
 // All sums have a fixed order. X is kept in both layouts (rows for A, its transpose for
 // B X), since the product takes both operands with the reduction axis contiguous.
 #include "tile_product.h"
@@ -215,8 +215,8 @@ __device__ __forceinline__ void put8(char* row, int k, const HiLo (&v)[8]) {   /
   *(f16x8*)(at + 64) = l;
 }
 
-// u / (|u| + eps) times S in both layouts. A workgroup takes 64 x 64 of [m][n]. Bound by HBM: 336 MB in
-// 61 us (5.5 TB/s) for 21 M elements with their momentum.
+// u / (|u| + eps) times S 2^j in both layouts. A workgroup takes 64 x 64 of [m][n]. Bound by HBM: 336 MB in
+// 59 to 69 us (5.7 to 4.9 TB/s) for 21 M elements with their momentum.
 __global__ __launch_bounds__(256) void muon_split_kernel(const Batch b) {
   __shared__ float tile[64][65];
   __shared__ double wsum[4];

@@ -111,7 +111,7 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_s
 class Plan(NamedTuple):
     """The n = T * k slots (t * k + j) sorted by expert: ``order`` int32 [n], the slot of each sorted row (-1
     behind the last expert's); ``position`` int32 [T, k], the sorted row of each slot (-1: no expert);
-    ``offsets`` int32 [E + 1], where each expert's rows begin."""
+    ``offsets`` int32 [E + 1], where each expert's rows begin (from 0 on, never falling)."""
     order: torch.Tensor
     position: torch.Tensor
     offsets: torch.Tensor

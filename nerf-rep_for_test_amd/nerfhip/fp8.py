@@ -130,8 +130,9 @@ def launch(x, weight, M, order, slots, offsets, bias, relu, out_dtype, who):
 def linear(x, weight, bias=None, relu=False, out_dtype=None):
     """y [.., N] = x [.., K] W^T (+ bias [N] float32, ReLU) with the activations rounded to
     8-bit blocks of 128; sums in float32, y in ``out_dtype`` (default: x's type). float32 results have
-    exact products, 16-bit ones the 8-bit matrix instruction's (1e-5 of a result's norm, below their
-    rounding). A block with a value that is not finite makes its row's outputs NaN. K up to 2^23."""
+    exact products, 16-bit ones the 8-bit matrix instruction's: 8 neighbouring products are added with 13 bits
+    below the largest, 1e-5 of a result's norm for values of usual spread and 7 * 2^-13 of the largest product at
+    most (1.75 half steps of float16, less than bfloat16's; ``out_dtype=torch.float32`` has none of it). A block with a value that is not finite makes its row's outputs NaN. K up to 2^23."""
     if not isinstance(weight, Fp8Weight) or weight.q.dim() != 2:
         raise ValueError("linear: weight must be an Fp8Weight of one matrix")
     if weight.k > 1 << 23:

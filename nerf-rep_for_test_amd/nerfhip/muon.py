@@ -150,6 +150,7 @@ class HipMuon(torch.optim.Optimizer):
     """Muon for the matrices that ``is_hidden_matrix`` names, HipAdam (same ``lr``, ``betas``, ``adam_eps``)
     for every other parameter; gradients clamped to [-``clip``, clip] on their way in (None: not). Matrices
     move by ``lr * muon_ratio`` times an orthogonal matrix: with Adam's usual 5e-4 and the ratio 40 by 0.02.
+    ``weight_decay`` is theirs alone.
 
     Group 0 holds the matrices (state: ``momentum_buffer``), group 1 the rest (HipAdam's state). lr is a
     device tensor in both (fill it to change it; the step then stays one captured graph). float32 contiguous
