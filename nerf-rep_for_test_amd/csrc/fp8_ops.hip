@@ -539,7 +539,7 @@ __device__ __forceinline__ bool find_further(const LinearArgs& a, int tile, int&
   const int at = __builtin_ctzll(met);
   int left = tile - __builtin_amdgcn_readlane(sum - mine, at);
   e = at * per;
-  for (int c; (c = tiles(e)) <= left; ++e) left -= c;   // (ends: that lane counted more than `left`)
+  for (int c; e + 1 < n && (c = tiles(e)) <= left; ++e) left -= c;   // (that lane counted more than `left`)
   e = __builtin_amdgcn_readfirstlane(e);
   expert_rows(a, e, m0, hi);
   m0 += 16 * (int64_t)(__builtin_amdgcn_readfirstlane(left) + 1);
@@ -547,12 +547,12 @@ __device__ __forceinline__ bool find_further(const LinearArgs& a, int tile, int&
 }
 
 // Few rows for each weight matrix: bound by the weights' bytes. A workgroup of 8 waves
-// takes 16 rows of x (blockIdx.y: the first 16 of each expert, then the further 16s of whatever
-// experts have them) and 16 TN weight rows;
-// the waves share the blocks of K between them, U at a time (all of their loads in flight),
-// read the weights straight into the matrix operands (16 rows x 128 B lines, no LDS) and
-// quantise the activations in registers (a row's block lies in 4 lanes), so one launch
-// reads each weight once for every 16 rows. The 8 partial sums are added in wave order.
+// takes 16 rows of x (blockIdx.y: the first 16 of each expert, then the further 16s of
+// whatever experts have them) and 16 TN weight rows; the waves share the blocks of K
+// between them, U at a time (all of their loads in flight), read the weights straight into
+// the matrix operands (16 rows x 128 B lines, no LDS) and quantise the activations in
+// registers (a row's block lies in 4 lanes), so one launch reads each weight once for every
+// 16 rows. The 8 partial sums are added in wave order.
 // Rows that a gate spreads unevenly (64 experts of 1024 x 2048, 1024 rows; 256 of 512 x 1024, 4096): all on one
 // expert 30 and 43 us (one workgroup walking them all: 415 and 990), at random 40 and 52 (48 and 47), evenly 30
 // and 41 (28 and 35: the further 16s' workgroups start and find nothing).
